@@ -19,19 +19,10 @@
 #include <stdexcept>
 #include <vector>
 
+#include "bind.h"
 #include "kernels.h"
 
 namespace zamd {
-
-#define HIP_CHECK(expr)                                              \
-  do {                                                               \
-    hipError_t _e = (expr);                                          \
-    TORCH_CHECK(_e == hipSuccess, "HIP error: ", hipGetErrorString(_e)); \
-  } while (0)
-
-static hipStream_t current_stream() {
-  return at::hip::getCurrentHIPStream().stream();
-}
 
 static const bf16* bf_ptr(const torch::Tensor& t) {
   TORCH_CHECK(t.scalar_type() == torch::kBFloat16, "expected bf16 tensor");
@@ -664,4 +655,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_fwd_threads", &zamd::set_fwd_threads);
   m.def("fused_bwd_active", &zamd::fused_bwd_ok);
   m.def("clear_graphs", &zamd::clear_graphs);
+  zamd::bind_glr(m);
 }

@@ -73,6 +73,35 @@ void launch_lstm_persistent_bwd(const bf16* dY, const bf16* rec,
                                 unsigned int* abort_flag, int T, int B,
                                 int H, hipStream_t stream);
 
+// glr.hip — gated linear recurrence. Strides are in elements; the last axis
+// is dense. c0, cT, dcT, dc0 and marks are f32 [.., B, H] and dense, but for
+// the state of launch_glr_step (cT, read and written), whose rows are c_b
+// apart.
+constexpr int GLR_MARK = 64;  // steps between two kept states
+enum class GlrType { F32, F16, BF16 };
+struct GlrArgs {
+  const void* gates = nullptr;  // [T, B, 4H]
+  int64_t gates_t = 0, gates_b = 0;
+  void* h = nullptr;            // [T, B, H]
+  int64_t h_t = 0, h_b = 0;
+  const void* dh = nullptr;     // [T, B, H]
+  int64_t dh_t = 0, dh_b = 0;
+  void* dgates = nullptr;       // [T, B, 4H]
+  int64_t dgates_t = 0, dgates_b = 0;
+  const float* c0 = nullptr;    // null: zeros
+  float* cT = nullptr;
+  int64_t c_b = 0;
+  const float* dcT = nullptr;   // null: zeros
+  float* dc0 = nullptr;         // null: not wanted
+  float* marks = nullptr;       // [ceil(T / GLR_MARK), B, H]; null: not kept
+  const void* lengths = nullptr;  // [B] int32 or int64; null: all T
+  bool lengths_64 = false;
+  int T = 0, B = 0, H = 0;
+};
+void launch_glr_fwd(const GlrArgs& a, GlrType type, hipStream_t stream);
+void launch_glr_bwd(const GlrArgs& a, GlrType type, hipStream_t stream);
+void launch_glr_step(const GlrArgs& a, GlrType type, hipStream_t stream);
+
 // elementwise.hip
 void launch_embedding_fwd(const bf16* W, const int64_t* idx, bf16* out,
                           int N, int H, hipStream_t stream);

@@ -13,7 +13,7 @@ The HIP kernel path lives in zaremba_amd/ops/hip_ops.py + csrc/.
 
 from __future__ import annotations
 
-from typing import List, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -65,6 +65,45 @@ def lstm_layer(
         h, c = lstm_step(x_t, h, c, W_x, W_h, b_x, b_h)
         outputs.append(h)
     return torch.stack(outputs), h, c
+
+
+# ---------------------------------------------------------------------------
+# Gated linear recurrence: the same cell without its recurrent product
+# ---------------------------------------------------------------------------
+
+def glr_step(gates: torch.Tensor, c: torch.Tensor
+             ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One step from [B, 4H] pre-activations, gate order (i, f, o, n), in
+    the state's type (float32 or wider); h in the gates' type."""
+    i, f, o, n = gates.to(c.dtype).chunk(4, 1)
+    c = torch.sigmoid(f) * c + torch.sigmoid(i) * torch.tanh(n)
+    return (torch.sigmoid(o) * torch.tanh(c)).to(gates.dtype), c
+
+
+def glr_layer(gates: torch.Tensor, c0: Optional[torch.Tensor] = None,
+              lengths: Optional[torch.Tensor] = None
+              ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The recurrence over [T, B, 4H]; row b ends after lengths[b] steps."""
+    T, B, H = gates.size(0), gates.size(1), gates.size(2) // 4
+    c = c0
+    if c is None:
+        wide = gates.dtype if gates.dtype == torch.float64 else torch.float32
+        c = torch.zeros(B, H, dtype=wide, device=gates.device)
+    if T == 0:
+        return gates.new_empty(0, B, H), c.clone()
+    outputs = []
+    for t, g in enumerate(gates.unbind(0)):
+        if lengths is not None:
+            live = (t < lengths)[:, None]
+            # what stands in a finished row must not reach a gradient
+            g = torch.where(live, g, torch.zeros_like(g))
+            h, new = glr_step(g, c)
+            h = torch.where(live, h, torch.zeros_like(h))
+            c = torch.where(live, new, c)
+        else:
+            h, c = glr_step(g, c)
+        outputs.append(h)
+    return torch.stack(outputs), c
 
 
 # ---------------------------------------------------------------------------
