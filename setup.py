@@ -22,6 +22,8 @@ ext = CUDAExtension(
         "zaremba_amd/csrc/lstm.hip",
         "zaremba_amd/csrc/lstm_persistent.hip",
         "zaremba_amd/csrc/elementwise.hip",
+        "zaremba_amd/csrc/adamw.hip",
+        "zaremba_amd/csrc/adamw_bind.hip",
         "zaremba_amd/csrc/glr.hip",
         "zaremba_amd/csrc/glr_bind.hip",
     ],

@@ -18,6 +18,7 @@ inline hipStream_t current_stream() {
   return at::hip::getCurrentHIPStream().stream();
 }
 
+void bind_adamw(py::module_& m);
 void bind_glr(py::module_& m);
 
 }  // namespace zamd

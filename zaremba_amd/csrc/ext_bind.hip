@@ -655,5 +655,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_fwd_threads", &zamd::set_fwd_threads);
   m.def("fused_bwd_active", &zamd::fused_bwd_ok);
   m.def("clear_graphs", &zamd::clear_graphs);
+  zamd::bind_adamw(m);
   zamd::bind_glr(m);
 }

@@ -102,6 +102,50 @@ void launch_glr_fwd(const GlrArgs& a, GlrType type, hipStream_t stream);
 void launch_glr_bwd(const GlrArgs& a, GlrType type, hipStream_t stream);
 void launch_glr_step(const GlrArgs& a, GlrType type, hipStream_t stream);
 
+// adamw.hip — AdamW over many tensors. The tensors of a launch travel in its
+// arguments (4 KB at most), so that no call copies a table to the device.
+constexpr int ADAMW_TENSORS = 48;
+constexpr int ADAMW_NORM_CHUNK = 65536;
+constexpr int ADAMW_CHUNK = 16384;
+struct AdamwTensor {
+  float* p;
+  const void* g;       // f32 or bf16
+  void* m;             // f32, or e4m3 codes
+  void* v;             // f32, or e4m3 codes of its root
+  float* m_scale;      // of 256 codes each
+  float* v_scale;
+  bf16* shadow;        // may be null
+  int64_t n;
+};
+struct AdamwTensors {
+  int count;
+  int begin[ADAMW_TENSORS + 1];       // first chunk of each tensor, and the end
+  int norm_begin[ADAMW_TENSORS + 1];  // the same in chunks of the norm
+  AdamwTensor t[ADAMW_TENSORS];
+};
+struct AdamwScalars {
+  int64_t* step;       // steps done; the norm's launch advances it
+  double lr, beta1, beta2, max_norm, grad_scale;
+  float b1, c1, b2, c2, eps, keep;  // c: 1 - b; keep: 1 - lr * decay
+  bool clip;
+};
+struct AdamwValues {  // of this step, left by the norm's launch
+  float rate, root;
+  unsigned step;
+};
+struct AdamwWork {
+  double* partials;    // [count] sums of squares
+  int count;
+  AdamwValues* values;
+  float* norm;
+};
+void launch_adamw_norm(const AdamwTensors& a, const AdamwScalars& s,
+                       bool bf16_grads, int first, const AdamwWork& w,
+                       hipStream_t stream);
+void launch_adamw_update(const AdamwTensors& a, const AdamwScalars& s,
+                         bool bf16_grads, bool bits8, bool tell,
+                         const AdamwWork& w, hipStream_t stream);
+
 // elementwise.hip
 void launch_embedding_fwd(const bf16* W, const int64_t* idx, bf16* out,
                           int N, int H, hipStream_t stream);

@@ -175,3 +175,96 @@ def clip_grad_and_sgd_(
             if p.grad is not None:
                 p.add_(p.grad, alpha=-lr * float(coef))
     return total_norm
+
+
+# ---------------------------------------------------------------------------
+# AdamW, states in 32 or in 8 bits (ops/adamw.py says what they are)
+# ---------------------------------------------------------------------------
+
+_E4M3_MAX, _TINY = 448.0, 2.0 ** -100
+
+
+def _blocks(x: torch.Tensor) -> torch.Tensor:
+    """[ceil(n / 256), 256] of the values, zeros behind the last."""
+    x = x.reshape(-1)
+    return torch.nn.functional.pad(x, (0, -x.numel() % 256)).view(-1, 256)
+
+
+def _e4m3_scales(x: torch.Tensor):
+    amax = x.abs().amax(1)
+    empty = amax < _TINY
+    zero = torch.zeros_like(amax)
+    return (torch.where(empty, zero, amax * (1 / _E4M3_MAX)),
+            torch.where(empty, zero, amax.reciprocal() * _E4M3_MAX)[:, None])
+
+
+def hash_uniform(index: torch.Tensor, step) -> torch.Tensor:
+    """Numbers in [0, 1) with 24 bits, from a 32-bit mixing hash."""
+    low = 0xFFFFFFFF
+    x = (index.long() * 0x9E3779B1 + step * 0x85EBCA77) & low
+    x = ((x ^ (x >> 16)) * 0x7FEB352D) & low
+    x = ((x ^ (x >> 15)) * 0x846CA68B) & low
+    return ((x ^ (x >> 16)) >> 8).float() * 2.0 ** -24
+
+
+def draw_e4m3(x: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
+    """Codes (uint8) of one of the two e4m3 values beside x >= 0, the upper
+    one where u < (x^2 - a^2) / (b^2 - a^2); 0 only for 0."""
+    x = x.clamp(max=_E4M3_MAX)
+    low = torch.where(x < 2.0 ** -6, (x * 512).int(),
+                      (x.view(torch.int32) >> 20) - 960).clamp(0, 126)
+    value = lambda c: c.to(torch.uint8).view(  # noqa: E731
+        torch.float8_e4m3fn).float()
+    a, b = value(low), value((low + 1).clamp(max=126))
+    up = u * (b * b - a * a) < x * x - a * a
+    return (low + torch.where(low == 0, x > 0, up)).clamp(
+        max=126).to(torch.uint8)
+
+
+def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps,
+                weight_decay, max_norm, grad_scale, exp_avg_scales,
+                exp_avg_sq_scales, shadows):
+    step += 1
+    t = int(step)
+    b1, b2 = betas
+    norm, scale = None, grad_scale
+    if max_norm is not None:
+        norm = torch.stack([g.double().square().sum() for g in grads]
+                           ).sum().sqrt() * grad_scale
+        scale = grad_scale * float(torch.clamp(max_norm / (norm + 1e-6),
+                                               max=1.0))
+        norm = norm.float()
+    rate, root = lr / (1 - b1 ** t), (1 - b2 ** t) ** -0.5
+    for k, p in enumerate(params):
+        n = p.numel()
+        g = grads[k].reshape(-1).float() * scale
+        if exp_avg_scales is None:
+            m, v = exp_avgs[k].view(-1), exp_avg_sqs[k].view(-1)
+        else:
+            m = (_blocks(exp_avgs[k].float())
+                 * exp_avg_scales[k][:, None]).view(-1)[:n]
+            v = (_blocks(exp_avg_sqs[k].float())
+                 * exp_avg_sq_scales[k][:, None]).view(-1)[:n].square()
+        m = m * b1 + g * (1 - b1)
+        v = v * b2 + g * g * (1 - b2)
+        r = v.sqrt()
+        flat = p.view(-1)
+        flat.copy_(flat * (1 - lr * weight_decay)
+                   - rate * (m / (r * root + eps)))
+        if shadows is not None and shadows[k] is not None:
+            shadows[k].copy_(p)
+        if exp_avg_scales is None:
+            exp_avgs[k].view(-1).copy_(m)
+            exp_avg_sqs[k].view(-1).copy_(v)
+            continue
+        mb, rb = _blocks(m), _blocks(r)
+        scales, inv = _e4m3_scales(mb)
+        exp_avg_scales[k].copy_(scales)
+        exp_avgs[k].copy_((mb * inv).view(-1)[:n].to(torch.float8_e4m3fn)
+                          .view(p.shape))
+        scales, inv = _e4m3_scales(rb)
+        exp_avg_sq_scales[k].copy_(scales)
+        u = hash_uniform(torch.arange(n, device=p.device), t)
+        codes = draw_e4m3((rb * inv).view(-1)[:n], u)
+        exp_avg_sqs[k].copy_(codes.view(torch.float8_e4m3fn).view(p.shape))
+    return norm

@@ -128,8 +128,7 @@ class GlrFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gates, c0, lengths):
         ctx.set_materialize_grads(False)
-        h, cT, marks = _C.ext().glr_forward(
-            gates, c0, lengths, any(ctx.needs_input_grad), None)
+        h, cT, marks = _C.ext().glr_forward(gates, c0, lengths, True, None)
         ctx.save_for_backward(gates, c0, lengths, marks)
         return h, cT
 
@@ -147,7 +146,10 @@ class GlrFn(torch.autograd.Function):
 def glr(gates, c0=None, lengths=None):
     """``(h, cT)``, differentiable in ``gates`` and ``c0``."""
     if not _eager(gates):
-        return GlrFn.apply(gates, c0, lengths)
+        if torch.is_grad_enabled() and (
+                gates.requires_grad or (c0 is not None and c0.requires_grad)):
+            return GlrFn.apply(gates, c0, lengths)
+        return _C.ext().glr_forward(gates, c0, lengths, False, None)[:2]
     _check_eager("glr", gates, 3, c0=c0)
     _check_lengths("glr", gates, lengths)
     return F_ref.glr_layer(gates, c0, lengths)
