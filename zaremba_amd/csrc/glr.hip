@@ -11,11 +11,25 @@
 //   do = dh tanh(c) o (1 - o)   dn = g i (1 - n^2)   dc0 = s(f_0) g_0
 //
 // From lengths[b] on, row b keeps its state, and its h and gate gradients
-// are zero whatever stands there.
+// are zero whatever stands there: such a step is (x, y) = (1, 0) by selects.
 //
-// One thread per channel walks the time axis. The forward pass keeps the
-// state before every GLR_MARK-th step, and the backward pass walks those
-// tiles from the last to the first and computes the states between again.
+// Steps compose: c -> A c + C with A = prod x and C the state that the steps
+// reach from zero. A block takes 64 channels and walks the time axis in tiles
+// of W * K steps, wave w holding K of them in registers: each wave finds its
+// (A, C), the waves exchange them through LDS, and each then runs its own
+// steps from the state that the waves before it leave. Data is read once,
+// 4 K loads of a wave are in flight together, and a step waits for no other
+// but through one exchange a tile (two in the backward pass).
+//
+// A lane has one channel, so that rows may have any length and alignment. Two
+// channels a lane, with loads twice as wide, measured 264 to 290 us against
+// 260 forward and 521 to 576 against 533 backward at 65536 x 1 x 1500: the
+// registers of twice the steps leave half the waves.
+
+#include <algorithm>
+#include <cmath>
+#include <cstdlib>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -23,90 +37,412 @@ namespace zamd {
 
 namespace {
 
-DEV_INLINE float sigmoid_f(float x) {
-  return __builtin_amdgcn_rcpf(1.f +
-                               __builtin_amdgcn_exp2f(x * -1.44269504089f));
-}
+constexpr float LOG2E = 1.44269504089f;
 
+DEV_INLINE float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+DEV_INLINE float rcp_f(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// exp and 1 / x are one instruction each, off by one unit of 2^-23. An
+// infinite exp(-x) gives rcp(inf) = 0, and exp(-inf) = 0 gives 1: closed and
+// open gates are exact.
+DEV_INLINE float sigmoid_f(float x) { return rcp_f(1.f + exp2_f(x * -LOG2E)); }
+
+// From exp(-2|x|) <= 1, which cannot overflow.
 DEV_INLINE float tanh_f(float x) {
-  const float e =
-      __builtin_amdgcn_exp2f(__builtin_fabsf(x) * -2.88539008178f);
-  return __builtin_copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x);
+  const float e = exp2_f(__builtin_fabsf(x) * (-2.f * LOG2E));
+  return __builtin_copysignf((1.f - e) * rcp_f(1.f + e), x);
 }
 
-DEV_INLINE int row_length(const GlrArgs& a, int b) {
-  if (!a.lengths) return a.T;
-  const int64_t n =
-      a.lengths_64 ? static_cast<const int64_t*>(a.lengths)[b]
-                   : (int64_t)static_cast<const int*>(a.lengths)[b];
-  return (int)(n < 0 ? 0 : n > a.T ? a.T : n);
+// s(x) tanh(y) with one reciprocal.
+DEV_INLINE float sigmoid_tanh(float x, float y) {
+  const float e = exp2_f(__builtin_fabsf(y) * (-2.f * LOG2E));
+  const float d = 1.f + e;
+  const float r = rcp_f(__builtin_fmaf(exp2_f(x * -LOG2E), d, d));
+  return __builtin_copysignf((1.f - e) * r, y);
 }
 
+// A uniform base and a lane's 32-bit byte offset.
 template <typename E>
-__global__ void glr_fwd_kernel(GlrArgs a) {
-  const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (id >= (int64_t)a.B * a.H) return;
-  const int b = (int)(id / a.H), j = (int)(id % a.H), H = a.H;
-  const int n_live = row_length(a, b);
-  const E* g = static_cast<const E*>(a.gates) + b * a.gates_b + j;
-  E* h = static_cast<E*>(a.h) + b * a.h_b + j;
-  float c = a.c0 ? a.c0[id] : 0.f;
-  for (int t = 0; t < a.T; ++t, g += a.gates_t, h += a.h_t) {
-    if (a.marks && t % GLR_MARK == 0)
-      a.marks[(int64_t)(t / GLR_MARK) * a.B * a.H + id] = c;
-    if (t < n_live) {
-      c = sigmoid_f((float)g[H]) * c +
-          sigmoid_f((float)g[0]) * tanh_f((float)g[3 * H]);
-      *h = (E)(sigmoid_f((float)g[2 * H]) * tanh_f(c));
-    } else {
-      *h = (E)0.f;
+DEV_INLINE const E& at(const E* base, unsigned offset) {
+  return *reinterpret_cast<const E*>(reinterpret_cast<const char*>(base) +
+                                     offset);
+}
+template <typename E>
+DEV_INLINE E& at(E* base, unsigned offset) {
+  return *reinterpret_cast<E*>(reinterpret_cast<char*>(base) + offset);
+}
+
+// One of a block's 64 channels: the b-th row of the launch, its j-th channel.
+struct Channel {
+  int first;      // row of the block's first lane
+  int row;        // this lane's row, less `first`
+  int j;
+  bool live;      // a lane behind the last channel repeats the block's first
+  int n_live;     // steps of the row
+  int64_t state;  // place in a [B, H]
+
+  DEV_INLINE Channel(const GlrArgs& a, int group) {
+    const int id0 = group * 64, id = id0 + lane_id();
+    live = id < a.rows * a.H;
+    const int b0 = id0 / a.H;
+    const int b = live ? id / a.H : b0;
+    first = a.row0 + b0;
+    row = b - b0;
+    j = (live ? id : id0) - b * a.H;
+    state = (int64_t)(first + row) * a.H + j;
+    n_live = a.T;
+    if (a.lengths) {
+      const int64_t n = a.lengths_64
+                            ? static_cast<const int64_t*>(a.lengths)[first + row]
+                            : static_cast<const int*>(a.lengths)[first + row];
+      n_live = (int)(n < 0 ? 0 : n > a.T ? a.T : n);
     }
   }
-  a.cT[id] = c;
+
+  // Rows of a block lie less than 4 GB apart (rows_per_launch sees to it).
+  template <typename E>
+  DEV_INLINE unsigned offset(int64_t row_stride) const {
+    return (unsigned)((row * row_stride + j) * sizeof(E));
+  }
+};
+
+template <typename E, int K>
+struct Gates {
+  E i[K], f[K], o[K], n[K];
+
+  // Steps [t0, t0 + K); those past T read the last one.
+  DEV_INLINE void load(const GlrArgs& a, const E* base, unsigned offset,
+                       int t0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const E* p = base + (int64_t)min(t0 + k, a.T - 1) * a.gates_t;
+      i[k] = at(p, offset);
+      f[k] = at(p + a.H, offset);
+      o[k] = at(p + 2 * (int64_t)a.H, offset);
+      n[k] = at(p + 3 * (int64_t)a.H, offset);
+    }
+  }
+
+  // Makes the steps from `stop` on stand for (x, y) = (1, 0).
+  DEV_INLINE void mask(int t0, int stop) {
+    if (__all(t0 + K <= stop)) return;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool on = t0 + k < stop;
+      i[k] = on ? i[k] : (E)-INFINITY;
+      f[k] = on ? f[k] : (E)INFINITY;
+      n[k] = on ? n[k] : (E)0.f;
+    }
+  }
+};
+
+// (A, C) of each wave of a block, for each channel.
+struct alignas(8) Pair {
+  float A, C;
+};
+
+// c through the pairs of the waves [from, to).
+DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
+  for (int q = from; q < to; ++q) {
+    const Pair p = pairs[q][lane_id()];
+    c = p.A * c + p.C;
+  }
+  return c;
 }
 
-template <typename E>
-__global__ void glr_bwd_kernel(GlrArgs a) {
-  const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (id >= (int64_t)a.B * a.H) return;
-  const int b = (int)(id / a.H), j = (int)(id % a.H), H = a.H;
-  const int n_live = row_length(a, b);
-  const E* g0 = static_cast<const E*>(a.gates) + b * a.gates_b + j;
-  const E* dh0 = static_cast<const E*>(a.dh) + b * a.dh_b + j;
-  E* d0 = static_cast<E*>(a.dgates) + b * a.dgates_b + j;
-  float carry = a.dcT ? a.dcT[id] : 0.f;
-  float before[GLR_MARK];
-  for (int tile = (a.T - 1) / GLR_MARK; tile >= 0; --tile) {
-    float c = a.marks[(int64_t)tile * a.B * a.H + id];
-    const int t0 = tile * GLR_MARK;
-    const int n = min(GLR_MARK, a.T - t0);
-    for (int k = 0; k < n; ++k) {
-      const E* g = g0 + (t0 + k) * a.gates_t;
-      before[k] = c;
-      if (t0 + k < n_live)
-        c = sigmoid_f((float)g[H]) * c +
-            sigmoid_f((float)g[0]) * tanh_f((float)g[3 * H]);
-    }
-    for (int k = n - 1; k >= 0; --k) {
-      const E* g = g0 + (t0 + k) * a.gates_t;
-      E* d = d0 + (t0 + k) * a.dgates_t;
-      if (t0 + k >= n_live) {
-        d[0] = d[H] = d[2 * H] = d[3 * H] = (E)0.f;
-        continue;
+// Where the channels make too few blocks for 256 CUs, the time axis is cut
+// into chunks of one tile, a block each, and the state is handed from chunk
+// to chunk while all of them are in flight. Slot r, the r-th chunk in the
+// order of the scan, has a word for each channel. It first publishes its
+// (A, C) there and, once it knows the state before it, the state behind it
+// instead, marked by A = -1. A wave looks back over the slots before its own,
+// DEPTH of them at a time, and composes their pairs until it meets a state.
+// A word says by itself whether it is there (all ones: not yet; no word that
+// is written is), so that no order between stores is needed, and words go
+// past the L2s, which do not see each other's writes.
+//
+// Blocks take their slots from a counter as they start. A block therefore
+// waits only for blocks that run already, and these only for earlier ones:
+// every wait ends, whatever the number of blocks that fit the chip. Polls are
+// bounded all the same; behind a bound that is reached the state is NaN.
+//
+// At T = 65536, B = 1, H = 1500, bf16 a chain takes 255 us forward (983 MB,
+// 3.9 TB/s of the 5.2 that a copy reaches) and 528 us backward (1770 MB, 3.4
+// TB/s); vector instructions take half of either, and without looking back at
+// all it is 248 and 516. Finding the (A, C) of long chunks in a launch of its
+// own, which reads three gates twice, took 360 and 680.
+constexpr unsigned ABSENT = 0xffffffffu;
+constexpr int MOST_POLLS = 1 << 22;
+constexpr int COUNTER_WORDS = GLR_COUNTER_WORDS;  // before the slots
+constexpr int DEPTH = 4;
+
+DEV_INLINE unsigned to_bits(float x) {  // any NaN but ABSENT
+  return x == x ? __builtin_bit_cast(unsigned, x) : 0x7fc00000u;
+}
+
+struct Chain {
+  unsigned* counter;
+  uint64_t* words;  // [chunks, B * H]: A above C
+  int64_t BH;
+
+  DEV_INLINE Chain(const GlrArgs& a)
+      : counter(reinterpret_cast<unsigned*>(a.work)),
+        words(a.work + COUNTER_WORDS), BH((int64_t)a.B * a.H) {}
+
+  DEV_INLINE int take_slot(int* lds) const {
+    if (threadIdx.x == 0)
+      *lds = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(*lds);
+  }
+
+  DEV_INLINE void publish(int slot, const Channel& ch, float A,
+                          float C) const {
+    if (!ch.live) return;
+    __hip_atomic_store(words + slot * BH + ch.state,
+                       (uint64_t)to_bits(A) << 32 | to_bits(C),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+
+  // The state before `slot`, found by one wave.
+  DEV_INLINE float look_back(int slot, const Channel& ch, float start) const {
+    float A = 1.f, C = 0.f;
+    bool met = !ch.live;
+    for (int back = slot - 1, polls = 0;;) {
+      uint64_t p[DEPTH];
+#pragma unroll
+      for (int q = 0; q < DEPTH; ++q)
+        p[q] = __hip_atomic_load(
+            words + (int64_t)max(back - q, 0) * BH + ch.state,
+            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      int seen = 0;
+#pragma unroll
+      for (int q = 0; q < DEPTH; ++q) {
+        if (back - q < 0 || polls >= MOST_POLLS) {
+          const float c = back - q < 0 ? start : __builtin_nanf("");
+          return met ? C : A * c + C;
+        }
+        if (!__all(met || (unsigned)(p[q] >> 32) != ABSENT)) break;
+        ++seen;
+        const float x = __builtin_bit_cast(float, (unsigned)(p[q] >> 32));
+        const float y = __builtin_bit_cast(float, (unsigned)p[q]);
+        C = met ? C : A * y + C;
+        A *= x;
+        met |= x < 0.f;
+        if (__all(met)) return C;
       }
-      const float i = sigmoid_f((float)g[0]), f = sigmoid_f((float)g[H]);
-      const float o = sigmoid_f((float)g[2 * H]), m = tanh_f((float)g[3 * H]);
-      const float tc = tanh_f(f * before[k] + i * m);
-      const float dh = (float)dh0[(t0 + k) * a.dh_t];
-      const float dc = dh * o * (1.f - tc * tc) + carry;
-      d[0] = (E)(dc * m * i * (1.f - i));
-      d[H] = (E)(dc * before[k] * f * (1.f - f));
-      d[2 * H] = (E)(dh * tc * o * (1.f - o));
-      d[3 * H] = (E)(dc * i * (1.f - m * m));
-      carry = f * dc;
+      back -= seen;
+      if (seen == 0) {
+        ++polls;
+        __builtin_amdgcn_s_sleep(1);
+      }
     }
   }
-  if (a.dc0) a.dc0[id] = carry;
+
+  // The state before `slot`, to all waves; the one behind it through `last`.
+  // The waves that look back go first: the blocks behind wait for them.
+  DEV_INLINE float hand_on(int slot, const Channel& ch, float A, float C,
+                           const float* start, float* lds, float* last,
+                           int w) const {
+    if (w == 0) {
+      __builtin_amdgcn_s_setprio(3);
+      publish(slot, ch, A, C);
+      const float c = look_back(slot, ch, start ? start[ch.state] : 0.f);
+      lds[lane_id()] = c;
+      const float behind = A * c + C;
+      publish(slot, ch, -1.f, behind);
+      if (last && ch.live) last[ch.state] = behind;
+      __builtin_amdgcn_s_setprio(0);
+    }
+    __syncthreads();
+    return lds[lane_id()];
+  }
+};
+
+// Nothing is there yet, and no slot taken.
+__global__ void glr_reset_kernel(uint4* work, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n)
+    work[i] = i < COUNTER_WORDS / 2 ? uint4{0, 0, 0, 0}
+                                    : uint4{ABSENT, ABSENT, ABSENT, ABSENT};
+}
+
+// W: waves of a block, in a chain and at most otherwise.
+template <typename E, int K, int W, bool CHAIN>
+__global__ __launch_bounds__(64 * W) void glr_fwd_kernel(GlrArgs a) {
+  __shared__ Pair lds[2][W][64];
+  __shared__ float handed[CHAIN ? 64 : 1];
+  __shared__ int taken;
+  const int waves = CHAIN ? W : blockDim.x / 64, lane = lane_id();
+  const int w = __builtin_amdgcn_readfirstlane(wave_id());
+  const int span = waves * K;
+  const int slot = CHAIN ? Chain(a).take_slot(&taken) : blockIdx.x;
+  const int chunk = CHAIN ? slot / a.groups : 0;
+  const Channel ch(a, slot - chunk * a.groups);
+  const E* g0 = static_cast<const E*>(a.gates) + ch.first * a.gates_b;
+  const unsigned g_off = ch.offset<E>(a.gates_b);
+  E* h0 = static_cast<E*>(a.h) + ch.first * a.h_b;
+  const unsigned h_off = ch.offset<E>(a.h_b);
+  const int begin = chunk * span;
+  const int end = CHAIN ? min(begin + span, a.T) : a.T;
+
+  Gates<E, K> g;
+  g.load(a, g0, g_off, begin + w * K);
+  float c = !CHAIN && a.c0 ? a.c0[ch.state] : 0.f;
+  for (int tile = begin, side = 0; tile < end; tile += span, side ^= 1) {
+    const int t0 = tile + w * K;
+    g.mask(t0, ch.n_live);
+    float x[K], y[K], A = 1.f, C = 0.f;
+    E o[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      o[k] = g.o[k];
+      x[k] = sigmoid_f((float)g.f[k]);
+      y[k] = sigmoid_tanh((float)g.i[k], (float)g.n[k]);
+      C = x[k] * C + y[k];
+      A *= x[k];
+    }
+    if (!CHAIN && tile + span < end) g.load(a, g0, g_off, t0 + span);
+    lds[side][w][lane] = {A, C};
+    __syncthreads();
+    if (CHAIN) {
+      if (w == 0)
+#pragma unroll
+        for (int q = 1; q < W; ++q) {
+          const Pair p = lds[0][q][lane];
+          C = p.A * C + p.C;
+          A *= p.A;
+        }
+      c = Chain(a).hand_on(chunk, ch, A, C, a.c0, handed,
+                           end == a.T ? a.cT : nullptr, w);
+    }
+    float now = c = compose(c, lds[side], 0, w);
+    if (a.marks && t0 % GLR_MARK == 0 && t0 < end && ch.live)
+      a.marks[(int64_t)(t0 / GLR_MARK) * a.B * a.H + ch.state] = now;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int t = t0 + k;
+      now = x[k] * now + y[k];
+      const float h = sigmoid_tanh((float)o[k], now);
+      if (t < end && ch.live)
+        at(h0 + t * a.h_t, h_off) = t < ch.n_live ? (E)h : (E)0.f;
+    }
+    if (!CHAIN) c = compose(c, lds[side], w, waves);
+  }
+  if (!CHAIN && w == 0 && ch.live) a.cT[ch.state] = c;
+}
+
+// Tiles begin at marks and are walked from the last.
+template <typename E, int K, int W, bool CHAIN>
+__global__ __launch_bounds__(64 * W) void glr_bwd_kernel(GlrArgs a) {
+  static_assert(K * W % GLR_MARK == 0);
+  __shared__ Pair lds[2][W][64];   // (A, C) of the states
+  __shared__ Pair back[2][W][64];  // (A, D) of their gradients, last first
+  __shared__ float handed[CHAIN ? 64 : 1];
+  __shared__ int taken;
+  const int waves = CHAIN ? W : blockDim.x / 64, lane = lane_id();
+  const int w = __builtin_amdgcn_readfirstlane(wave_id());
+  const int rw = waves - 1 - w;
+  const int span = waves * K;
+  const int slot = CHAIN ? Chain(a).take_slot(&taken) : blockIdx.x;
+  const int order = CHAIN ? slot / a.groups : 0;
+  const Channel ch(a, slot - order * a.groups);
+  const E* g0 = static_cast<const E*>(a.gates) + ch.first * a.gates_b;
+  const unsigned g_off = ch.offset<E>(a.gates_b);
+  const E* dh0 = static_cast<const E*>(a.dh) + ch.first * a.dh_b;
+  const unsigned dh_off = ch.offset<E>(a.dh_b);
+  E* d0 = static_cast<E*>(a.dgates) + ch.first * a.dgates_b;
+  const unsigned d_off = ch.offset<E>(a.dgates_b);
+  const int begin = CHAIN ? (a.chunks - 1 - order) * span : 0;
+  const int end = CHAIN ? min(begin + span, a.T) : a.T;
+
+  float carry = !CHAIN && a.dcT ? a.dcT[ch.state] : 0.f;
+  int side = 0;
+  for (int tile = begin + (end - 1 - begin) / span * span; tile >= begin;
+       tile -= span, side ^= 1) {
+    const int t0 = tile + w * K;
+    Gates<E, K> g;
+    g.load(a, g0, g_off, t0);
+    E dh[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      dh[k] = at(dh0 + (int64_t)min(t0 + k, a.T - 1) * a.dh_t, dh_off);
+    float c = a.marks[(int64_t)(tile / GLR_MARK) * a.B * a.H + ch.state];
+
+    const int stop = ch.n_live;
+    g.mask(t0, stop);
+    if (!__all(t0 + K <= stop)) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        g.o[k] = t0 + k < stop ? g.o[k] : (E)0.f;
+        dh[k] = t0 + k < stop ? dh[k] : (E)0.f;
+      }
+    }
+    float i[K], f[K], n[K], A = 1.f, C = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      i[k] = sigmoid_f((float)g.i[k]);
+      f[k] = sigmoid_f((float)g.f[k]);
+      n[k] = tanh_f((float)g.n[k]);
+      C = f[k] * C + i[k] * n[k];
+      A *= f[k];
+    }
+    lds[side][w][lane] = {A, C};
+    __syncthreads();
+    c = compose(c, lds[side], 0, w);
+    // Forward again through the own steps; u is what a step adds to g, and
+    // D what the steps hand back from a gradient of zero behind them. The
+    // output gate's gradient needs no more and is written at once.
+    float before[K], u[K], D = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int t = t0 + k;
+      before[k] = c;
+      c = f[k] * c + i[k] * n[k];
+      const float tc = tanh_f(c);
+      const float o = sigmoid_f((float)g.o[k]);
+      const float od = o * (float)dh[k];
+      u[k] = od * (1.f - tc * tc);
+      if (t < end && ch.live)
+        at(d0 + t * a.dgates_t + 2 * (int64_t)a.H, d_off) =
+            t < stop ? (E)(od * tc * (1.f - o)) : (E)0.f;
+    }
+#pragma unroll
+    for (int k = K - 1; k >= 0; --k) D = f[k] * (D + u[k]);
+    back[side][rw][lane] = {A, D};
+    __syncthreads();
+    if (CHAIN) {
+      float whole = 1.f, sum = 0.f;
+      if (w == 0)
+#pragma unroll
+        for (int q = 0; q < W; ++q) {
+          const Pair p = back[0][q][lane];
+          sum = p.A * sum + p.C;
+          whole *= p.A;
+        }
+      carry = Chain(a).hand_on(order, ch, whole, sum, a.dcT, handed,
+                               begin == 0 ? a.dc0 : nullptr, w);
+    }
+    float now = carry = compose(carry, back[side], 0, rw);
+#pragma unroll
+    for (int k = K - 1; k >= 0; --k) {
+      const int t = t0 + k;
+      const float dc = now + u[k], dci = dc * i[k], dcf = dc * f[k];
+      now = dcf;
+      if (t < end && ch.live) {
+        const bool on = t < stop;
+        E* d = d0 + t * a.dgates_t;
+        at(d, d_off) = on ? (E)(dci * n[k] * (1.f - i[k])) : (E)0.f;
+        at(d + a.H, d_off) =
+            on ? (E)(dcf * before[k] * (1.f - f[k])) : (E)0.f;
+        at(d + 3 * (int64_t)a.H, d_off) =
+            on ? (E)(dci * (1.f - n[k] * n[k])) : (E)0.f;
+      }
+    }
+    if (!CHAIN) carry = compose(carry, back[side], rw, waves);
+  }
+  if (!CHAIN && w == 0 && ch.live) a.dc0[ch.state] = carry;
 }
 
 template <typename E>
@@ -117,10 +453,10 @@ __global__ void glr_step_kernel(GlrArgs a) {
   const E* g = static_cast<const E*>(a.gates) + b * a.gates_b + j;
   float* cp = a.cT + b * a.c_b + j;
   const float c = sigmoid_f((float)g[H]) * *cp +
-                  sigmoid_f((float)g[0]) * tanh_f((float)g[3 * H]);
+                  sigmoid_tanh((float)g[0], (float)g[3 * H]);
   *cp = c;
   static_cast<E*>(a.h)[b * a.h_b + j] =
-      (E)(sigmoid_f((float)g[2 * H]) * tanh_f(c));
+      (E)sigmoid_tanh((float)g[2 * H], c);
 }
 
 template <typename F>
@@ -132,22 +468,80 @@ void by_type(GlrType type, F f) {
   }
 }
 
+constexpr int STEPS = 8;        // of a wave in a tile
+constexpr int LOOP_WAVES = 8;   // at most
+constexpr int FWD_WAVES = 16;   // of a chain's blocks: the counter gives
+constexpr int BWD_WAVES = 8;    // a slot every 14 ns; 16 spill backward
+
+// Rows of one launch: all, unless rows lie so far apart that those of a block
+// do not fit a lane's 32-bit offset; then one.
+int rows_per_launch(const GlrArgs& a, int size) {
+  const int64_t most =
+      std::max(std::max(std::abs(a.gates_b), std::abs(a.h_b)),
+               std::max(std::abs(a.dh_b), std::abs(a.dgates_b)));
+  const int64_t apart = 63 / a.H + 1;  // rows from a block's first to last
+  return (apart * most + 4 * (int64_t)a.H) * size < (int64_t)1 << 32 ? a.B : 1;
+}
+
+// A loop over the tiles of 64 steps costs about 2.3 us a tile (4 backward)
+// as long as few blocks share the memory; a chain about 12 us, and then what
+// its bytes take at 3.3 to 3.8 TB/s, where a loop of many blocks reaches 4.4.
+// Measured, forward / backward in us, loop against chain: 24 groups of 64
+// channels, 4 tiles 12 / 19 against 12 / 13, 16 tiles 37 / 63 against 13 / 19;
+// 234 groups, 8 tiles 26 / 56 against 33 / 56; 375 groups, 16 tiles 80 / 171
+// against 73 / 146; 512 groups, 32 tiles 148 / 276 against 150 / 300.
+bool is_chain(const GlrArgs& a) {
+  const int tiles = cdiv(a.T, LOOP_WAVES * STEPS);
+  return a.groups < 448 && tiles > 4 + a.groups / 32;
+}
+
+GlrArgs planned(GlrArgs a, bool back, int size) {
+  a.rows = rows_per_launch(a, size);
+  a.groups = cdiv((int64_t)a.rows * a.H, 64);
+  a.chunks = is_chain(a)
+                 ? cdiv(a.T, (back ? BWD_WAVES : FWD_WAVES) * STEPS)
+                 : 0;
+  return a;
+}
+
+template <bool BACK, typename E>
+void launch(const GlrArgs& args, hipStream_t stream) {
+  constexpr int CHAIN_W = BACK ? BWD_WAVES : FWD_WAVES;
+  GlrArgs a = planned(args, BACK, sizeof(E));
+  for (a.row0 = 0; a.row0 < a.B; a.row0 += a.rows) {
+    if (a.chunks) {
+      const int64_t n = glr_work_words(args, BACK, sizeof(E)) / 2;
+      hipLaunchKernelGGL(glr_reset_kernel, dim3(cdiv(n, 256)), dim3(256), 0,
+                         stream, reinterpret_cast<uint4*>(a.work), n);
+      auto kernel = BACK ? glr_bwd_kernel<E, STEPS, CHAIN_W, true>
+                         : glr_fwd_kernel<E, STEPS, CHAIN_W, true>;
+      hipLaunchKernelGGL(kernel, dim3(a.groups * a.chunks),
+                         dim3(64 * CHAIN_W), 0, stream, a);
+    } else {
+      auto kernel = BACK ? glr_bwd_kernel<E, STEPS, LOOP_WAVES, false>
+                         : glr_fwd_kernel<E, STEPS, LOOP_WAVES, false>;
+      hipLaunchKernelGGL(kernel, dim3(a.groups),
+                         dim3(64 * std::min(LOOP_WAVES, cdiv(a.T, STEPS))), 0,
+                         stream, a);
+    }
+  }
+}
+
 }  // namespace
 
+int64_t glr_work_words(const GlrArgs& args, bool back, int size) {
+  const GlrArgs a = planned(args, back, size);
+  if (!a.chunks) return 0;
+  const int64_t n = COUNTER_WORDS + (int64_t)a.chunks * a.B * a.H;
+  return n + (n & 1);
+}
+
 void launch_glr_fwd(const GlrArgs& a, GlrType type, hipStream_t stream) {
-  const int grid = cdiv((int64_t)a.B * a.H, 64);
-  by_type(type, [&](auto e) {
-    hipLaunchKernelGGL(glr_fwd_kernel<decltype(e)>, dim3(grid), dim3(64), 0,
-                       stream, a);
-  });
+  by_type(type, [&](auto e) { launch<false, decltype(e)>(a, stream); });
 }
 
 void launch_glr_bwd(const GlrArgs& a, GlrType type, hipStream_t stream) {
-  const int grid = cdiv((int64_t)a.B * a.H, 64);
-  by_type(type, [&](auto e) {
-    hipLaunchKernelGGL(glr_bwd_kernel<decltype(e)>, dim3(grid), dim3(64), 0,
-                       stream, a);
-  });
+  by_type(type, [&](auto e) { launch<true, decltype(e)>(a, stream); });
 }
 
 void launch_glr_step(const GlrArgs& a, GlrType type, hipStream_t stream) {

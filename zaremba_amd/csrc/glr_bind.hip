@@ -37,7 +37,7 @@ void check_gates(const Tensor& gates, int64_t dims, const char* op) {
               ": the last axis of gates holds the 4 gates, got ",
               gates.size(-1), " values");
   const int64_t B = gates.size(-2), H = gates.size(-1) / 4;
-  TORCH_CHECK(B * H < std::numeric_limits<int>::max() &&
+  TORCH_CHECK(B * H < std::numeric_limits<int>::max() - 64 &&
               (dims == 2 || gates.size(0) < std::numeric_limits<int>::max()),
               op, ": sizes ", gates.sizes(), " are too large");
 }
@@ -95,6 +95,16 @@ void set_sizes(GlrArgs& a, const Tensor& gates) {
 
 int64_t mark_count(int64_t T) { return (T + GLR_MARK - 1) / GLR_MARK; }
 
+// A workspace of this call alone: the caching allocator keeps those of other
+// streams and of captured graphs apart.
+Tensor workspace(GlrArgs& a, bool back, const Tensor& gates) {
+  const int64_t words = glr_work_words(a, back, (int)gates.element_size());
+  if (!words) return Tensor();
+  Tensor work = torch::empty({words}, gates.options().dtype(torch::kInt64));
+  a.work = reinterpret_cast<uint64_t*>(work.data_ptr<int64_t>());
+  return work;
+}
+
 std::tuple<Tensor, Tensor, OptTensor> glr_forward(
     const Tensor& gates_in, const OptTensor& c0_in, const OptTensor& lengths,
     bool training, const OptTensor& out) {
@@ -137,6 +147,7 @@ std::tuple<Tensor, Tensor, OptTensor> glr_forward(
   a.h_b = h.stride(1);
   a.cT = cT.data_ptr<float>();
   if (marks) a.marks = marks->data_ptr<float>();
+  Tensor work = workspace(a, false, gates);
   launch_glr_fwd(a, type, current_stream());
   HIP_CHECK(hipGetLastError());
   return {h, cT, marks};
@@ -209,6 +220,7 @@ std::tuple<Tensor, Tensor> glr_backward(
   a.dgates_b = dgates.stride(1);
   a.marks = marks.data_ptr<float>();
   a.dc0 = dc0.data_ptr<float>();
+  Tensor work = workspace(a, true, gates);
   launch_glr_bwd(a, type, current_stream());
   HIP_CHECK(hipGetLastError());
   return {dgates, dc0};

@@ -77,7 +77,8 @@ void launch_lstm_persistent_bwd(const bf16* dY, const bf16* rec,
 // is dense. c0, cT, dcT, dc0 and marks are f32 [.., B, H] and dense, but for
 // the state of launch_glr_step (cT, read and written), whose rows are c_b
 // apart.
-constexpr int GLR_MARK = 64;  // steps between two kept states
+constexpr int GLR_MARK = 32;  // steps between two kept states
+constexpr int GLR_COUNTER_WORDS = 32;
 enum class GlrType { F32, F16, BF16 };
 struct GlrArgs {
   const void* gates = nullptr;  // [T, B, 4H]
@@ -97,7 +98,13 @@ struct GlrArgs {
   const void* lengths = nullptr;  // [B] int32 or int64; null: all T
   bool lengths_64 = false;
   int T = 0, B = 0, H = 0;
+  uint64_t* work = nullptr;  // glr_work_words of them, this call's own
+  // set by the launchers: the rows of a launch, its blocks of 64 channels
+  // and chunks of time
+  int row0 = 0, rows = 0, groups = 0, chunks = 0;
 };
+// Words of 64 bits that a call needs for itself; size: of a gate in bytes.
+int64_t glr_work_words(const GlrArgs& a, bool back, int size);
 void launch_glr_fwd(const GlrArgs& a, GlrType type, hipStream_t stream);
 void launch_glr_bwd(const GlrArgs& a, GlrType type, hipStream_t stream);
 void launch_glr_step(const GlrArgs& a, GlrType type, hipStream_t stream);
