@@ -12,9 +12,19 @@
 // of the step and the element's place in its tensor. A root that is not zero
 // is never rounded to zero, so that no update divides by eps alone.
 //
+// Two launches: the sum of squares (the norm is of all gradients, so they are
+// read twice), and the update, in which each block first adds up the partial
+// sums while its first loads are in flight. At 66.0M parameters with bf16
+// shadows they take 427 us in 32 bits (2.25 GB with the second reading, 5.26
+// TB/s, what a copy reaches), and 300 us in 8 bits (1.45 GB, 4.8 TB/s), where
+// vector instructions, some 86 a value, are busy 85 % of the update's time.
+//
 // Sums and the arithmetic of an update are in the order of the formulas, each
 // product and sum rounded (no contraction), and the norm is summed in 64 bits
 // over fixed chunks: the same inputs give the same bits.
+#include <algorithm>
+#include <type_traits>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -25,14 +35,75 @@ namespace zamd {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int QBLOCK = 256;  // elements that share a scale
+constexpr int WAVES = THREADS / 64;
+constexpr int QBLOCK = 256;  // elements that share a scale: 4 a lane
 constexpr float E4M3_MAX = 448.f;
 constexpr float TINY = 0x1p-100f;
+
+// Four neighbours at any alignment of the element.
+template <typename T>
+struct Quad {
+  T v[4];
+};
+
+template <typename T>
+DEV_INLINE Quad<T> load4(const T* p) {
+  Quad<T> x;
+  __builtin_memcpy(&x, p, sizeof x);
+  return x;
+}
+
+template <typename T>
+DEV_INLINE void store4(T* p, const Quad<T>& x) {
+  __builtin_memcpy(p, &x, sizeof x);
+}
+
+// Of the first `n` of them; the others read as zeros and are not written.
+template <typename T>
+DEV_INLINE Quad<T> load_some(const T* p, int n) {
+  Quad<T> x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x.v[e] = e < n ? p[e] : T(0);
+  return x;
+}
+
+template <typename T>
+DEV_INLINE void store_some(T* p, const Quad<T>& x, int n) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < n) p[e] = x.v[e];
+}
+
+// The tensor that chunk `c` of a launch belongs to.
+DEV_INLINE int tensor_of(const int* begin, int count, int c) {
+  int lo = 0, hi = count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (begin[mid] <= c) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// How many of a tensor's n values chunk number `c` has. The comparison is in 32
+// bits: of a minimum in 64 bits of values that a block shares the compiler
+// has selected the wrong one (s_cselect after a v_cmp that leaves scc alone).
+DEV_INLINE int chunk_length(int64_t n, int c, int chunk) {
+  const int64_t left = n - (int64_t)c * chunk;  // at least 1
+  const unsigned low = (unsigned)left;
+  return (left >> 32) != 0 || low > (unsigned)chunk ? chunk : (int)low;
+}
+
+DEV_INLINE double block_sum(double x, double* lds) {
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_down(x, off, 64);
+  if (lane_id() == 0) lds[wave_id()] = x;
+  __syncthreads();
+  return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+}
 
 template <typename G>
 __global__ __launch_bounds__(THREADS) void adamw_norm_kernel(
     AdamwTensors a, AdamwScalars s, int first, AdamwWork w) {
-  __shared__ double part[THREADS / 64];
+  __shared__ double lds[WAVES];
   if (first + blockIdx.x == 0 && threadIdx.x == 0) {
     const int64_t t = *s.step + 1;
     *s.step = t;
@@ -47,37 +118,50 @@ __global__ __launch_bounds__(THREADS) void adamw_norm_kernel(
     w.values->step = (unsigned)t;
   }
   if (!s.clip) return;
-  int k = 0;
-  while (k + 1 < a.count && a.norm_begin[k + 1] <= (int)blockIdx.x) ++k;
-  const int64_t at =
-      (int64_t)((int)blockIdx.x - a.norm_begin[k]) * ADAMW_NORM_CHUNK;
-  const int n = (int)min((int64_t)ADAMW_NORM_CHUNK, a.t[k].n - at);
-  const G* g = static_cast<const G*>(a.t[k].g) + at;
   double sum = 0;
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const double x = (double)(float)g[i];
-    sum += x * x;
+  for (int c = blockIdx.x; c < a.norm_begin[a.count]; c += gridDim.x) {
+    const int k = tensor_of(a.norm_begin, a.count, c);
+    const int rel = c - a.norm_begin[k];
+    const int n = chunk_length(a.t[k].n, rel, ADAMW_NORM_CHUNK);
+    const G* g =
+        static_cast<const G*>(a.t[k].g) + (int64_t)rel * ADAMW_NORM_CHUNK;
+    constexpr int R = ADAMW_NORM_CHUNK / THREADS / 4;
+    if (n == ADAMW_NORM_CHUNK) {
+      Quad<G> x[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        x[r] = load4(g + (r * THREADS + threadIdx.x) * 4);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const double y = (double)(float)x[r].v[e];
+          sum = __builtin_fma(y, y, sum);  // y * y is exact
+        }
+    } else {
+      for (int i = threadIdx.x * 4; i < n; i += THREADS * 4) {
+        const Quad<G> x = load_some(g + i, n - i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const double y = (double)(float)x.v[e];
+          sum = __builtin_fma(y, y, sum);
+        }
+      }
+    }
   }
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_down(sum, off, 64);
-  if (lane_id() == 0) part[wave_id()] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0)
-    w.partials[first + blockIdx.x] =
-        (part[0] + part[1]) + (part[2] + part[3]);
+  sum = block_sum(sum, lds);
+  if (threadIdx.x == 0) w.partials[first + blockIdx.x] = sum;
 }
 
 // What the gradients are multiplied by: in every block the same sum, in the
 // same order.
 DEV_INLINE float clip_scale(const AdamwScalars& s, const AdamwWork& w,
                             bool tell) {
-  __shared__ double part[THREADS / 64];
+  __shared__ double lds[WAVES];
   if (!s.clip) return (float)s.grad_scale;
   double sum = 0;
   for (int i = threadIdx.x; i < w.count; i += THREADS) sum += w.partials[i];
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_down(sum, off, 64);
-  if (lane_id() == 0) part[wave_id()] = sum;
-  __syncthreads();
-  sum = (part[0] + part[1]) + (part[2] + part[3]);
+  sum = block_sum(sum, lds);
   const double norm = __builtin_sqrt(sum) * s.grad_scale;
   if (tell && threadIdx.x == 0) *w.norm = (float)norm;
   double coef = s.max_norm / (norm + 1e-6);
@@ -85,136 +169,271 @@ DEV_INLINE float clip_scale(const AdamwScalars& s, const AdamwWork& w,
   return (float)(coef * s.grad_scale);
 }
 
-DEV_INLINE float hash_uniform(unsigned index, unsigned step) {
-  unsigned x = index * 0x9E3779B1u + step * 0x85EBCA77u;
+constexpr unsigned HASH_INDEX = 0x9E3779B1u, HASH_STEP = 0x85EBCA77u;
+
+DEV_INLINE float hash_uniform(unsigned x) {
   x = (x ^ (x >> 16)) * 0x7FEB352Du;
   x = (x ^ (x >> 15)) * 0x846CA68Bu;
   return (float)((x ^ (x >> 16)) >> 8) * 0x1p-24f;
 }
 
-DEV_INLINE float from_e4m3(unsigned code) {
-  return __builtin_amdgcn_cvt_f32_fp8((int)code, 0);
-}
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-DEV_INLINE unsigned to_e4m3(float x) {
-  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xff;
+// sqrt(x) of x >= 0, rounded to the nearest: the hardware's root is within
+// one unit, and a root s is the nearest where x lies between s times its two
+// neighbours (Tuckerman's test). The library's own form scales x < 2^-96
+// first; here such a root may be a unit off, beside one that is never under
+// eps. As bits, 0 and infinity have neighbours that are NaN, or too small to
+// change the test.
+DEV_INLINE float sqrt_f(float x) {
+  const float s = __builtin_amdgcn_sqrtf(x);
+  const unsigned u = __builtin_bit_cast(unsigned, s);
+  const float down = __builtin_bit_cast(float, u - 1);
+  const float up = __builtin_bit_cast(float, u + 1);
+  const float r = __builtin_fmaf(-down, s, x) <= 0.f ? down : s;
+  return __builtin_fmaf(-up, s, x) > 0.f ? up : r;
 }
 
 // One of the two codes beside x (0 <= x), so that x^2 is right in the mean.
-DEV_INLINE unsigned draw_e4m3(float x, unsigned index, unsigned step) {
-  x = x > E4M3_MAX ? E4M3_MAX : x;
-  const unsigned low =
-      x < 0x1p-6f ? (unsigned)(x * 512.f)
-                  : (__builtin_bit_cast(unsigned, x) >> 20) - 960u;
-  if (low == 0) return x > 0 ? 1 : 0;
-  if (low >= 126) return 126;
-  const float a = from_e4m3(low), b = from_e4m3(low + 1);
-  const float aa = a * a;
-  return hash_uniform(index, step) * (b * b - aa) < x * x - aa ? low + 1
-                                                               : low;
+// hashed: step * C2 + index * C1 of the element.
+DEV_INLINE unsigned draw_e4m3(float x, unsigned hashed) {
+  // less than the least code is drawn as the least code; 0 is put back below
+  const float y = __builtin_fminf(__builtin_fmaxf(x, 0x1p-9f), E4M3_MAX);
+  unsigned low = (__builtin_bit_cast(unsigned, y) >> 20) - 960u;
+  low = y < 0x1p-6f ? (unsigned)(y * 512.f) : low;
+  const f32x2 ab =
+      __builtin_amdgcn_cvt_pk_f32_fp8((int)(low * 257u + 256u), false);
+  const float aa = ab.x * ab.x;
+  // above 126 is a NaN, and no number less than one
+  low += hash_uniform(hashed) * (ab.y * ab.y - aa) < y * y - aa;
+  return x > 0.f ? low : 0;
 }
 
-// The largest magnitude of a wave; a NaN is the largest of all.
-DEV_INLINE float wave_amax(float x) {
-  unsigned u = __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const unsigned o = __shfl_xor(u, off, 64);
-    u = u > o ? u : o;
+// The largest of a wave, in every lane.
+DEV_INLINE unsigned wave_max(unsigned u) {
+#define ZAMD_MAX_DPP(ctrl)                                                  \
+  {                                                                         \
+    const unsigned o =                                                      \
+        (unsigned)__builtin_amdgcn_update_dpp(0, (int)u, ctrl, 0xf, 0xf,    \
+                                              false);                       \
+    u = u > o ? u : o;                                                      \
   }
-  return __builtin_bit_cast(float, u);
+  ZAMD_MAX_DPP(0x111)  // row_shr:1
+  ZAMD_MAX_DPP(0x112)  // row_shr:2
+  ZAMD_MAX_DPP(0x114)  // row_shr:4
+  ZAMD_MAX_DPP(0x118)  // row_shr:8
+  ZAMD_MAX_DPP(0x142)  // row_bcast:15
+  ZAMD_MAX_DPP(0x143)  // row_bcast:31
+#undef ZAMD_MAX_DPP
+  return (unsigned)__builtin_amdgcn_readlane((int)u, 63);
 }
+
+DEV_INLINE float from_lane(float x, int lane) {
+  return __builtin_bit_cast(
+      float,
+      __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+}
+
+// As bits a NaN is larger than any number.
+DEV_INLINE unsigned magnitude(float x) {
+  return __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
+}
+
+// Where a block's chunk of a tensor begins: uniform, so that a lane needs a
+// 32-bit offset only.
+template <typename G, typename S>
+struct Chunk {
+  float* p;
+  const G* g;
+  S* m;
+  S* v;
+  float* ms;
+  float* vs;
+  bf16* shadow;
+  unsigned hashed;  // of the chunk's first element
+
+  DEV_INLINE Chunk(const AdamwTensor& x, int64_t at)
+      : p(x.p + at), g(static_cast<const G*>(x.g) + at),
+        m(static_cast<S*>(x.m) + at), v(static_cast<S*>(x.v) + at),
+        ms(x.m_scale + at / QBLOCK), vs(x.v_scale + at / QBLOCK),
+        shadow(x.shadow ? x.shadow + at : nullptr),
+        hashed((unsigned)at * HASH_INDEX) {}
+};
+
+// 256 elements of a chunk, 4 a lane.
+template <typename G, bool BITS8>
+struct Block {
+  using S = typename std::conditional<BITS8, uint8_t, float>::type;
+  Quad<float> p;
+  Quad<G> g;
+  Quad<S> m, v;
+  float ms, vs;
+
+  // q: the block's first element. n: those left from this lane's on; 4 or
+  // more throughout where WHOLE.
+  template <bool WHOLE>
+  DEV_INLINE void load(const Chunk<G, S>& x, int q, int n) {
+    const unsigned i = q + lane_id() * 4;
+    if (WHOLE) {
+      g = load4(x.g + i);
+      p = load4(x.p + i);
+      m = load4(x.m + i);
+      v = load4(x.v + i);
+    } else {
+      g = load_some(x.g + i, n);
+      p = load_some(x.p + i, n);
+      m = load_some(x.m + i, n);
+      v = load_some(x.v + i, n);
+    }
+    if (BITS8) {
+      ms = x.ms[q / QBLOCK];
+      vs = x.vs[q / QBLOCK];
+    }
+  }
+
+  template <bool WHOLE>
+  DEV_INLINE void update(const Chunk<G, S>& x, int q, int n,
+                         const AdamwScalars& s, float coef, float rate,
+                         float root) {
+    const unsigned i = q + lane_id() * 4;
+    Quad<float> m1, r1;
+    Quad<bf16> sh;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float gr = (float)g.v[e] * coef;
+      float m0, v0;
+      if constexpr (BITS8) {
+        const float r0 = unpack(v, e) * vs;
+        m0 = unpack(m, e) * ms;
+        v0 = r0 * r0;
+      } else {
+        m0 = m.v[e];
+        v0 = v.v[e];
+      }
+      m1.v[e] = m0 * s.b1 + gr * s.c1;
+      const float v1 = v0 * s.b2 + gr * gr * s.c2;
+      // In 8 bits the arithmetic is what bounds the kernel: one reciprocal,
+      // off by one unit of 2^-23, in place of a division's dozen of steps.
+      r1.v[e] = BITS8 ? sqrt_f(v1) : __builtin_sqrtf(v1);
+      const float d = r1.v[e] * root + s.eps;
+      const float move = BITS8 ? m1.v[e] * __builtin_amdgcn_rcpf(d)
+                               : m1.v[e] / d;
+      p.v[e] = p.v[e] * s.keep - rate * move;
+      sh.v[e] = (bf16)p.v[e];
+      if constexpr (!BITS8) {
+        m.v[e] = m1.v[e];
+        v.v[e] = v1;
+      }
+    }
+    if constexpr (BITS8) {
+      unsigned um = 0, ur = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        um = max(um, magnitude(m1.v[e]));
+        ur = max(ur, magnitude(r1.v[e]));
+      }
+      // half the wave divides for m, half for r
+      const unsigned am = wave_max(um), ar = wave_max(ur);
+      const float most =
+          __builtin_bit_cast(float, lane_id() < 32 ? am : ar);
+      const bool empty = most < TINY;
+      const float inv = empty ? 0.f : 1.f / most * E4M3_MAX;
+      const float scale = empty ? 0.f : most * (1.f / E4M3_MAX);
+      if ((lane_id() & 31) == 0)
+        (lane_id() ? x.vs : x.ms)[q / QBLOCK] = scale;
+      const float im = from_lane(inv, 0), ir = from_lane(inv, 32);
+      int c = __builtin_amdgcn_cvt_pk_fp8_f32(m1.v[0] * im, m1.v[1] * im, 0,
+                                              false);
+      c = __builtin_amdgcn_cvt_pk_fp8_f32(m1.v[2] * im, m1.v[3] * im, c,
+                                          true);
+      __builtin_memcpy(&m, &c, 4);
+      const unsigned hashed = x.hashed + i * HASH_INDEX;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v.v[e] =
+            (uint8_t)draw_e4m3(r1.v[e] * ir, hashed + e * HASH_INDEX);
+    }
+    if (WHOLE) {
+      store4(x.p + i, p);
+      store4(x.m + i, m);
+      store4(x.v + i, v);
+      if (x.shadow) store4(x.shadow + i, sh);
+    } else {
+      store_some(x.p + i, p, n);
+      store_some(x.m + i, m, n);
+      store_some(x.v + i, v, n);
+      if (x.shadow) store_some(x.shadow + i, sh, n);
+    }
+  }
+
+  static DEV_INLINE float unpack(const Quad<uint8_t>& q, int e) {
+    int c;
+    __builtin_memcpy(&c, &q, 4);
+    const f32x2 x = e < 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(c, false)
+                          : __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+    return e & 1 ? x.y : x.x;
+  }
+};
 
 template <typename G, bool BITS8>
 __global__ __launch_bounds__(THREADS) void adamw_update_kernel(
     AdamwTensors a, AdamwScalars s, bool tell, AdamwWork w) {
+  constexpr int AHEAD = 2;  // blocks of 256 that a wave has in flight
+  constexpr int STRIDE = WAVES * QBLOCK;
+  // From the last chunk to the first: the gradients that the norm read last
+  // are those that a cache may still hold.
+  const int c = a.begin[a.count] - 1 - (int)blockIdx.x;
+  const int k = tensor_of(a.begin, a.count, c);
+  const int rel = c - a.begin[k];
+  const int n = chunk_length(a.t[k].n, rel, ADAMW_CHUNK);
+  Chunk<G, typename Block<G, BITS8>::S> x(a.t[k], (int64_t)rel * ADAMW_CHUNK);
+  const int whole = n / QBLOCK * QBLOCK;
+  const int wave = __builtin_amdgcn_readfirstlane(wave_id());
+
+  int q = wave * QBLOCK;
+  Block<G, BITS8> b[AHEAD];
+#pragma unroll
+  for (int r = 0; r < AHEAD; ++r)
+    if (q + r * STRIDE < whole)
+      b[r].template load<true>(x, q + r * STRIDE, 4);
   const float coef = clip_scale(s, w, tell && blockIdx.x == 0);
   const float rate = w.values->rate, root = w.values->root;
-  const unsigned step = w.values->step;
-  int k = 0;
-  while (k + 1 < a.count && a.begin[k + 1] <= (int)blockIdx.x) ++k;
-  const AdamwTensor& x = a.t[k];
-  const int64_t at = (int64_t)((int)blockIdx.x - a.begin[k]) * ADAMW_CHUNK;
-  const int64_t end = min(at + (int64_t)ADAMW_CHUNK, x.n);
-  const G* gp = static_cast<const G*>(x.g);
-  for (int64_t q = at + wave_id() * QBLOCK; q < end;
-       q += THREADS / 64 * QBLOCK) {
-    float m[4], r[4];
-    const int64_t i0 = q + lane_id() * 4;
-    float ms = 0, vs = 0;
-    if (BITS8) {
-      ms = x.m_scale[q / QBLOCK];
-      vs = x.v_scale[q / QBLOCK];
-    }
+  x.hashed += w.values->step * HASH_STEP;
+  for (; q < whole; q += AHEAD * STRIDE) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t i = i0 + e;
-      m[e] = r[e] = 0;
-      if (i >= end) continue;
-      const float g = (float)gp[i] * coef;
-      float m0, v0;
-      if (BITS8) {
-        m0 = from_e4m3(static_cast<uint8_t*>(x.m)[i]) * ms;
-        const float r0 = from_e4m3(static_cast<uint8_t*>(x.v)[i]) * vs;
-        v0 = r0 * r0;
-      } else {
-        m0 = static_cast<float*>(x.m)[i];
-        v0 = static_cast<float*>(x.v)[i];
-      }
-      m[e] = m0 * s.b1 + g * s.c1;
-      const float v = v0 * s.b2 + g * g * s.c2;
-      r[e] = __builtin_sqrtf(v);
-      const float p =
-          x.p[i] * s.keep - rate * (m[e] / (r[e] * root + s.eps));
-      x.p[i] = p;
-      if (x.shadow) x.shadow[i] = (bf16)p;
-      if (!BITS8) {
-        static_cast<float*>(x.m)[i] = m[e];
-        static_cast<float*>(x.v)[i] = v;
-      }
+    for (int r = 0; r < AHEAD; ++r) {
+      const int i = q + r * STRIDE;
+      if (i >= whole) break;
+      Block<G, BITS8> now = b[r];
+      if (i + AHEAD * STRIDE < whole)
+        b[r].template load<true>(x, i + AHEAD * STRIDE, 4);
+      now.template update<true>(x, i, 4, s, coef, rate, root);
     }
-    if (BITS8) {
-      float am = m[0], ar = r[0];
-      {
-        unsigned um = 0, ur = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          um = max(um, __builtin_bit_cast(unsigned, m[e]) & 0x7fffffffu);
-          ur = max(ur, __builtin_bit_cast(unsigned, r[e]) & 0x7fffffffu);
-        }
-        am = wave_amax(__builtin_bit_cast(float, um));
-        ar = wave_amax(__builtin_bit_cast(float, ur));
-      }
-      const float im = am < TINY ? 0.f : 1.f / am * E4M3_MAX;
-      const float ir = ar < TINY ? 0.f : 1.f / ar * E4M3_MAX;
-      if (lane_id() == 0) {
-        x.m_scale[q / QBLOCK] = am < TINY ? 0.f : am * (1.f / E4M3_MAX);
-        x.v_scale[q / QBLOCK] = ar < TINY ? 0.f : ar * (1.f / E4M3_MAX);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t i = i0 + e;
-        if (i >= end) continue;
-        static_cast<uint8_t*>(x.m)[i] = (uint8_t)to_e4m3(m[e] * im);
-        static_cast<uint8_t*>(x.v)[i] =
-            (uint8_t)draw_e4m3(r[e] * ir, (unsigned)i, step);
-      }
-    }
+  }
+  // what is left of the tensor behind its last whole 256
+  if (whole < n && wave == whole / QBLOCK % WAVES) {
+    const int left = n - whole - lane_id() * 4;
+    Block<G, BITS8> last;
+    last.template load<false>(x, whole, left);
+    last.template update<false>(x, whole, left, s, coef, rate, root);
   }
 }
 
 }  // namespace
 
+// Every block of the update reads the partial sums of all of these: 512 to
+// 1536 measured the same, 4096 8 % more at 66M parameters in 8 bits.
+int adamw_norm_blocks(const AdamwTensors& a, int launches) {
+  return std::max(1, std::min(a.norm_begin[a.count], 1024 / launches));
+}
+
 void launch_adamw_norm(const AdamwTensors& a, const AdamwScalars& s,
-                       bool bf16_grads, int first, const AdamwWork& w,
-                       hipStream_t stream) {
-  const int blocks = s.clip ? a.norm_begin[a.count] : 1;
-  if (bf16_grads)
-    hipLaunchKernelGGL(adamw_norm_kernel<bf16>, dim3(blocks), dim3(THREADS),
-                       0, stream, a, s, first, w);
-  else
-    hipLaunchKernelGGL(adamw_norm_kernel<float>, dim3(blocks), dim3(THREADS),
-                       0, stream, a, s, first, w);
+                       bool bf16_grads, int first, int blocks,
+                       const AdamwWork& w, hipStream_t stream) {
+  auto kernel =
+      bf16_grads ? adamw_norm_kernel<bf16> : adamw_norm_kernel<float>;
+  hipLaunchKernelGGL(kernel, dim3(s.clip ? blocks : 1), dim3(THREADS), 0,
+                     stream, a, s, first, w);
 }
 
 void launch_adamw_update(const AdamwTensors& a, const AdamwScalars& s,

@@ -31,7 +31,7 @@ void check_one(const Tensor& x, const Tensor& p, const char* name, size_t k,
               "] must be contiguous");
 }
 
-Tensor adamw_step_(const Tensors& params, const Tensors& grads,
+OptTensor adamw_step_(const Tensors& params, const Tensors& grads,
                    const Tensors& ms, const Tensors& vs, const Tensor& step,
                    double lr, double beta1, double beta2, double eps,
                    double weight_decay, c10::optional<double> max_norm,
@@ -132,11 +132,9 @@ Tensor adamw_step_(const Tensors& params, const Tensors& grads,
     TORCH_CHECK(written[k - 1].second <= written[k].first,
                 "adamw_step_: parameters, states or shadows share memory");
 
-  // chunks of the norm in all launches
-  int64_t chunks = 0;
-  for (const auto& t : all)
-    chunks += (t.n + ADAMW_NORM_CHUNK - 1) / ADAMW_NORM_CHUNK;
-  TORCH_CHECK(chunks < std::numeric_limits<int>::max() / 8,
+  int64_t total = 0;
+  for (const auto& t : all) total += t.n;
+  TORCH_CHECK(total / ADAMW_NORM_CHUNK < std::numeric_limits<int>::max() / 8,
               "adamw_step_: too many values");
   AdamwScalars s = {};
   s.step = step.data_ptr<int64_t>();
@@ -153,17 +151,6 @@ Tensor adamw_step_(const Tensors& params, const Tensors& grads,
   s.eps = (float)eps;
   s.keep = (float)(1 - lr * weight_decay);
 
-  // One workspace a call: the caching allocator keeps those of captured
-  // graphs apart.
-  Tensor norm = torch::zeros({}, first.options());
-  Tensor room = torch::empty({chunks + 2}, first.options().dtype(
-                                               torch::kFloat64));
-  AdamwWork w;
-  w.values = reinterpret_cast<AdamwValues*>(room.data_ptr<double>());
-  w.partials = room.data_ptr<double>() + 2;
-  w.count = s.clip ? (int)chunks : 0;
-  w.norm = norm.data_ptr<float>();
-
   std::vector<AdamwTensors> launches;
   for (size_t k = 0; k < all.size(); k += ADAMW_TENSORS) {
     AdamwTensors a = {};
@@ -179,25 +166,41 @@ Tensor adamw_step_(const Tensors& params, const Tensors& grads,
     launches.push_back(a);
   }
   if (launches.empty()) launches.push_back(AdamwTensors{});  // step alone
+
+  // One workspace a call: the caching allocator keeps those of captured
+  // graphs apart.
+  int partials = 0;
+  for (const auto& a : launches)
+    partials += adamw_norm_blocks(a, (int)launches.size());
+  Tensor room = torch::empty({partials + 3}, first.options().dtype(
+                                                 torch::kFloat64));
+  Tensor norm;
+  AdamwWork w;
+  w.values = reinterpret_cast<AdamwValues*>(room.data_ptr<double>());
+  w.partials = room.data_ptr<double>() + 2;
+  w.count = s.clip ? partials : 0;
+  w.norm = nullptr;
+  if (s.clip) {
+    norm = all.empty() ? torch::zeros({}, first.options())
+                       : torch::empty({}, first.options());
+    w.norm = norm.data_ptr<float>();
+  }
   const auto stream = current_stream();
   int done = 0;
-  for (size_t k = 0; k < launches.size(); ++k) {
-    const AdamwTensors& a = launches[k];
-    if (k == 0 || s.clip) {
-      AdamwScalars one = s;
-      if (a.count == 0) one.clip = false;
-      launch_adamw_norm(a, one, grad == torch::kBFloat16, done, w, stream);
-      HIP_CHECK(hipGetLastError());
-      done += a.norm_begin[a.count];
-    }
+  for (const auto& a : launches) {
+    if (done && !s.clip) break;
+    const int blocks = adamw_norm_blocks(a, (int)launches.size());
+    launch_adamw_norm(a, s, grad == torch::kBFloat16, done, blocks, w, stream);
+    HIP_CHECK(hipGetLastError());
+    done += blocks;
   }
-  for (size_t k = 0; k < launches.size(); ++k) {
-    if (launches[k].count == 0) continue;
-    launch_adamw_update(launches[k], s, grad == torch::kBFloat16, bits8,
-                        k == 0, w, stream);
+  for (const auto& a : launches) {
+    if (a.count == 0) continue;
+    launch_adamw_update(a, s, grad == torch::kBFloat16, bits8,
+                        &a == &launches[0], w, stream);
     HIP_CHECK(hipGetLastError());
   }
-  return norm;
+  return s.clip ? OptTensor(norm) : OptTensor();
 }
 
 }  // namespace

@@ -112,8 +112,8 @@ void launch_glr_step(const GlrArgs& a, GlrType type, hipStream_t stream);
 // adamw.hip — AdamW over many tensors. The tensors of a launch travel in its
 // arguments (4 KB at most), so that no call copies a table to the device.
 constexpr int ADAMW_TENSORS = 48;
-constexpr int ADAMW_NORM_CHUNK = 65536;
-constexpr int ADAMW_CHUNK = 16384;
+constexpr int ADAMW_NORM_CHUNK = 8192;  // values of a tensor at a time
+constexpr int ADAMW_CHUNK = 4096;       // values of a block, of one tensor
 struct AdamwTensor {
   float* p;
   const void* g;       // f32 or bf16
@@ -146,9 +146,10 @@ struct AdamwWork {
   AdamwValues* values;
   float* norm;
 };
+int adamw_norm_blocks(const AdamwTensors& a, int launches);
 void launch_adamw_norm(const AdamwTensors& a, const AdamwScalars& s,
-                       bool bf16_grads, int first, const AdamwWork& w,
-                       hipStream_t stream);
+                       bool bf16_grads, int first, int blocks,
+                       const AdamwWork& w, hipStream_t stream);
 void launch_adamw_update(const AdamwTensors& a, const AdamwScalars& s,
                          bool bf16_grads, bool bits8, bool tell,
                          const AdamwWork& w, hipStream_t stream);

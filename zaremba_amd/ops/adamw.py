@@ -69,11 +69,10 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr,
     if len(params) == 0:
         raise RuntimeError("adamw_step_: no parameters")
     if params[0].is_cuda and not _C.force_eager_env():
-        norm = _C.ext().adamw_step_(
+        return _C.ext().adamw_step_(
             params, grads, exp_avgs, exp_avg_sqs, step, lr, betas[0],
             betas[1], eps, weight_decay, max_norm, grad_scale,
             exp_avg_scales, exp_avg_sq_scales, shadows)
-        return norm if max_norm is not None else None
     lists = [grads, exp_avgs, exp_avg_sqs] + [
         x for x in (exp_avg_scales, exp_avg_sq_scales, shadows)
         if x is not None]
