@@ -29,7 +29,7 @@ from zaremba_amd.ensemble_eval import (ensemble_perplexity,
 from zaremba_amd.models.lstm_lm import Model
 from zaremba_amd.parallel import dist as zdist
 
-from main import setdevice  # same device policy/messages
+from main import make_optimizer, setdevice  # same policies/messages
 
 
 def build_parser():
@@ -70,6 +70,17 @@ def build_parser():
                              "to gpu if one exists, falls back to cpu otherwise.")
     # Additive flags.
     parser.add_argument("--seed", type=int, default=None)
+    parser.add_argument("--cell", type=str, choices=["lstm", "glr"],
+                        default="lstm",
+                        help="The recurrent layer: the LSTM, or the gated "
+                             "linear recurrence (the same gates without the "
+                             "recurrent product).")
+    parser.add_argument("--optimizer", type=str,
+                        choices=["sgd", "adamw", "adamw8bit"], default="sgd",
+                        help="Clipped SGD as in the reference, or AdamW with "
+                             "states in 32 or in 8 bits.")
+    parser.add_argument("--weight_decay", type=float, default=0.01,
+                        help="AdamW's decoupled weight decay.")
     parser.add_argument("--engine", type=str,
                         choices=["auto", "hip", "eager"], default="auto")
     parser.add_argument("--dtype", type=str, choices=["fp32", "bf16"],
@@ -100,14 +111,15 @@ def train_one(args, vocab_size, data, model_num, jsonl_path=None):
         engine = "eager"
         os.environ["ZAREMBA_AMD_FORCE_EAGER"] = "1"
     model = Model(vocab_size, args.hidden_size, args.layer_num, args.dropout,
-                  args.winit, args.lstm_type, engine=engine)
+                  args.winit, args.lstm_type, engine=engine, cell=args.cell)
     model.to(args.device)
     if args.device.type == "cuda" and args.dtype == "bf16":
         model.hip().set_compute_dtype(torch.bfloat16)
     trainer.train(data, model, args.total_epochs, args.factor_epoch,
                   args.learning_rate, args.factor, args.max_grad_norm,
                   args.batch_size, log_every=800, model_num=model_num,
-                  jsonl_path=jsonl_path, is_rank0=True)
+                  jsonl_path=jsonl_path, is_rank0=True,
+                  optimizer=make_optimizer(args, model))
     return model
 
 

@@ -3,8 +3,9 @@
 main.py (same flags, defaults and console output; reference main.py:10-41),
 running on the MI355X-native zaremba_amd framework.
 
-Additive flags (absent from the reference): --seed, --engine, --dtype,
---data, --data_dir, --save, --resume, --jsonl. Multi-GPU data parallelism:
+Additive flags (absent from the reference): --seed, --cell, --optimizer,
+--weight_decay, --engine, --dtype, --data, --data_dir, --save, --resume,
+--jsonl. Multi-GPU data parallelism:
 launch with `python -m torch.distributed.run --nproc-per-node N
 --master-addr 127.0.0.1 main.py ...` — one rank per GPU over RCCL/xGMI.
 """
@@ -58,6 +59,17 @@ def build_parser():
     # Additive flags.
     parser.add_argument("--seed", type=int, default=None,
                         help="Random seed (the reference has none).")
+    parser.add_argument("--cell", type=str, choices=["lstm", "glr"],
+                        default="lstm",
+                        help="The recurrent layer: the LSTM, or the gated "
+                             "linear recurrence (the same gates without the "
+                             "recurrent product).")
+    parser.add_argument("--optimizer", type=str,
+                        choices=["sgd", "adamw", "adamw8bit"], default="sgd",
+                        help="Clipped SGD as in the reference, or AdamW with "
+                             "states in 32 or in 8 bits.")
+    parser.add_argument("--weight_decay", type=float, default=0.01,
+                        help="AdamW's decoupled weight decay.")
     parser.add_argument("--engine", type=str,
                         choices=["auto", "hip", "eager"], default="auto",
                         help="Compute path: fused HIP kernels (GPU) or eager "
@@ -116,6 +128,15 @@ def load_data(args):
     return zdata.data_init(args.data_dir)
 
 
+def make_optimizer(args, model):
+    """None for the reference's SGD, which the trainer does itself."""
+    if args.optimizer == "sgd":
+        return None
+    from zaremba_amd.ops.adamw import AdamW
+    return AdamW(model.parameters(), weight_decay=args.weight_decay,
+                 bits=8 if args.optimizer == "adamw8bit" else 32)
+
+
 def main():
     args = build_parser().parse_args()
     if args.engine == "hip" and args.dtype == "fp32":
@@ -144,11 +165,13 @@ def main():
     tst = zdata.minibatch(tst_raw, args.batch_size, args.seq_length)
 
     start_epoch, start_lr = 0, args.learning_rate
+    resumed = None
     if args.resume and os.path.exists(args.resume):
         from zaremba_amd.checkpoint import (build_model_from_checkpoint,
                                             restore_rng)
         model, payload = build_model_from_checkpoint(args.resume, engine=args.engine)
         start_epoch = payload["epoch"]
+        resumed = payload
         # Restore the RNG streams so a resumed run's dropout masks and
         # any data draws continue the unbroken run's sequence.
         restore_rng(payload)
@@ -157,7 +180,7 @@ def main():
     else:
         model = Model(vocab_size, args.hidden_size, args.layer_num,
                       args.dropout, args.winit, args.lstm_type,
-                      engine=args.engine)
+                      engine=args.engine, cell=args.cell)
     if args.device.type == "cuda" and args.dtype == "fp32":
         # engine auto (hip+fp32 was rejected at parse time): fp32 compute
         # on GPU = the eager engine
@@ -173,11 +196,19 @@ def main():
         from zaremba_amd.parallel.bucketer import GradBucketer
         dp = GradBucketer(model)
 
+    optimizer = make_optimizer(args, model)
+    if resumed is not None and optimizer is not None:
+        if "optimizer" not in resumed:
+            raise SystemExit(f"{args.resume} holds no optimizer states: it "
+                             "was not saved under --optimizer "
+                             f"{args.optimizer}")
+        optimizer.load_state_dict(resumed["optimizer"])
+
     trainer.train(
         (trn, vld, tst), model, args.total_epochs, args.factor_epoch,
         start_lr, args.factor, args.max_grad_norm, args.batch_size,
         jsonl_path=args.jsonl, save_path=args.save, start_epoch=start_epoch,
-        dp=dp, is_rank0=zdist.is_rank0(),
+        dp=dp, is_rank0=zdist.is_rank0(), optimizer=optimizer,
     )
     zdist.finalize()
 

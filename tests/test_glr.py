@@ -480,3 +480,23 @@ def test_offsets_past_32_bits():
     h2, cT2, marks = G.glr_forward(src, c0, training=True)
     d2, dc02 = G.glr_backward(dh, dcT, src, c0, marks)
     assert torch.equal(h, h2) and torch.equal(d, d2)
+
+
+@GPU
+@pytest.mark.parametrize("T", [3, 400])
+def test_rows_further_apart_than_an_offset_reaches(T):
+    """Rows of the batch over 4 GB apart, in a loop and in a chain."""
+    B, H = 3, 40
+    apart = (1 << 31) + 24
+    room = torch.empty(2 * apart + T * 4 * H, dtype=torch.bfloat16,
+                       device="cuda")
+    gates = room.as_strided((T, B, 4 * H), (4 * H, apart, 1))
+    src, c0, dh, dcT, lengths = make(T, B, H, torch.bfloat16, "cuda",
+                                     ragged=True)
+    gates.copy_(src)
+    h, cT, marks = G.glr_forward(gates, c0, lengths, training=True)
+    d, dc0 = G.glr_backward(dh, dcT, gates, c0, marks, lengths)
+    h2, cT2, marks2 = G.glr_forward(src, c0, lengths, training=True)
+    d2, dc02 = G.glr_backward(dh, dcT, src, c0, marks2, lengths)
+    for a, b in ((h, h2), (cT, cT2), (d, d2), (dc0, dc02)):
+        near(a, b.double().cpu(), 16.0, "far rows")

@@ -1,0 +1,313 @@
+"""The gated linear recurrence and AdamW together, as a model's training and
+evaluation use them."""
+
+import json
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from zaremba_amd import trainer
+from zaremba_amd.checkpoint import (build_model_from_checkpoint,
+                                    save_checkpoint)
+from zaremba_amd.models.lstm_lm import Model
+from zaremba_amd.ops.adamw import AdamW
+from zaremba_amd.ops import functional as F_ref
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+GPU = pytest.mark.gpu
+
+
+def model(engine="eager", vocab=60, hidden=24, layers=2, dropout=0.0,
+          seed=0, **kw):
+    torch.manual_seed(seed)
+    return Model(vocab, hidden, layers, dropout, 0.1, engine=engine,
+                 cell="glr", **kw)
+
+
+def batch(T, B, vocab, seed=1, device="cpu"):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randint(0, vocab, (T, B), generator=gen).to(device),
+            torch.randint(0, vocab, (T, B), generator=gen).to(device))
+
+
+def test_unknown_cell_is_refused():
+    with pytest.raises(ValueError, match="cell"):
+        Model(10, 4, 1, 0.0, 0.1, cell="gru")
+
+
+def test_model_is_its_formulas():
+    """Scores of the model against the cell written out step by step."""
+    m = model().double()
+    x, y = batch(7, 3, 60)
+    states = [(h.double(), c.double()) for h, c in m.state_init(3)]
+    scores, states = m(x, states)
+    cur = m.embed.W[x]
+    for k, layer in enumerate(m.rnns):
+        c, out = torch.zeros(3, 24, dtype=torch.float64), []
+        for t in range(7):
+            g = cur[t] @ layer.W_x.t() + layer.b_x
+            i, f, o, n = (g[:, j * 24:(j + 1) * 24] for j in range(4))
+            c = torch.sigmoid(f) * c + torch.sigmoid(i) * torch.tanh(n)
+            out.append(torch.sigmoid(o) * torch.tanh(c))
+        cur = torch.stack(out)
+        # a dozen roundings of 2^-53 of numbers under 1
+        assert float((states[k][1] - c).detach().abs().max()) < 1e-14
+    want = cur.view(21, -1) @ m.fc.W.t() + m.fc.b
+    assert float((scores - want).detach().abs().max()) < 1e-13
+
+
+def test_windows_carry_the_state():
+    m = model().eval()
+    x, _ = batch(12, 3, 60)
+    with torch.no_grad():
+        whole, _ = m(x, m.state_init(3))
+        states, parts = m.state_init(3), []
+        for a, b in ((0, 5), (5, 6), (6, 12)):
+            s, states = m(x[a:b], states)
+            parts.append(s)
+    # the projection's sums may run in another order: 24 terms under 1
+    assert float((torch.cat(parts) - whole).abs().max()) < 24 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_checkpoint_carries_cell_and_states(tmp_path, bits):
+    m = model()
+    opt = AdamW(m.parameters(), bits=bits)
+
+    def steps(mm, oo, seeds):
+        mm.train()
+        for s in seeds:
+            x, y = batch(6, 3, 60, seed=s)
+            mm.zero_grad()
+            scores, _ = mm(x, mm.state_init(3))
+            trainer.nll_loss(scores, y).backward()
+            trainer.adamw_step(mm, oo, 1e-2, 5.0)
+
+    steps(m, opt, (1, 2))
+    path = str(tmp_path / "m.pt")
+    save_checkpoint(path, m, extra={"optimizer": opt.state_dict()})
+    m2, payload = build_model_from_checkpoint(path, engine="eager")
+    assert m2.cell == "glr"
+    opt2 = AdamW(m2.parameters(), bits=bits)
+    opt2.load_state_dict(payload["optimizer"])
+    steps(m, opt, (3, 4))
+    steps(m2, opt2, (3, 4))
+    for a, b in zip(m.parameters(), m2.parameters()):
+        assert torch.equal(a, b)
+
+
+def test_checkpoint_without_cell_is_an_lstm(tmp_path):
+    m = Model(20, 8, 1, 0.0, 0.1, engine="eager")
+    path = str(tmp_path / "m.pt")
+    save_checkpoint(path, m)
+    payload = torch.load(path, weights_only=False)
+    del payload["model_args"]["cell"]
+    torch.save(payload, path)
+    m2, _ = build_model_from_checkpoint(path, engine="eager")
+    assert m2.cell == "lstm"
+
+
+def run_cli(args):
+    return subprocess.run([sys.executable] + args, cwd=REPO, timeout=300,
+                          capture_output=True, text=True)
+
+
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("optimizer", ["adamw", "adamw8bit"])
+def test_cli_trains_saves_and_resumes(tmp_path, optimizer):
+    ck, jl = str(tmp_path / "m.pt"), str(tmp_path / "m.jsonl")
+    args = ["main.py", "--device", "cpu", "--data",
+            "synthetic:vocab=40,tokens=3000", "--hidden_size", "16",
+            "--layer_num", "2", "--seq_length", "8", "--batch_size", "4",
+            "--dropout", "0.1", "--seed", "1", "--cell", "glr",
+            "--optimizer", optimizer, "--learning_rate", "0.005"]
+    r = run_cli(args + ["--total_epochs", "1", "--save", ck, "--jsonl", jl])
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert "Test set perplexity" in r.stdout
+    assert any(json.loads(line)["event"] == "final" for line in open(jl))
+    r = run_cli(args + ["--total_epochs", "2", "--resume", ck])
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert "Resumed from" in r.stdout
+    # states of the other kind are refused
+    other = "adamw" if optimizer == "adamw8bit" else "adamw8bit"
+    args[args.index(optimizer)] = other
+    r = run_cli(args + ["--total_epochs", "2", "--resume", ck])
+    assert r.returncode != 0 and "bits" in r.stderr
+
+
+@pytest.mark.timeout(300)
+def test_cli_refuses_states_that_were_not_saved(tmp_path):
+    ck = str(tmp_path / "m.pt")
+    args = ["main.py", "--device", "cpu", "--data",
+            "synthetic:vocab=40,tokens=3000", "--hidden_size", "16",
+            "--layer_num", "1", "--seq_length", "8", "--batch_size", "4"]
+    r = run_cli(args + ["--total_epochs", "1", "--save", ck])
+    assert r.returncode == 0, r.stderr[-2000:]
+    r = run_cli(args + ["--total_epochs", "2", "--resume", ck,
+                        "--optimizer", "adamw"])
+    assert r.returncode != 0 and "no optimizer states" in r.stderr
+
+
+@pytest.mark.timeout(300)
+def test_ensemble_cli(tmp_path):
+    r = run_cli(["ensemble.py", "--device", "cpu", "--data",
+                 "synthetic:vocab=40,tokens=3000", "--hidden_size", "16",
+                 "--layer_num", "1", "--seq_length", "8", "--batch_size",
+                 "4", "--total_epochs", "1", "--ensemble_num", "2", "--cell",
+                 "glr", "--optimizer", "adamw", "--learning_rate", "0.01",
+                 "--save_dir", str(tmp_path)])
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert "Test set perplexity of 2 averaged models" in r.stdout
+
+
+# ---------------------------------------------------------------------------
+# HIP engine
+# ---------------------------------------------------------------------------
+
+def rel(a, b):
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    return float((a - b).norm() / b.norm())
+
+
+# bf16 on the way: embedding, gates and h of two layers, weights, scores'
+# operands. Each rounding is off by 2^-9 / sqrt(3) of its value in the mean,
+# a dozen of them add up to 0.4 %, and the gates' slopes at most double that;
+# a gradient passes as many roundings again.
+SCORES, GRADS = 1e-2, 2e-2
+
+
+@GPU
+@pytest.mark.parametrize("T,B,H", [(35, 20, 200), (9, 40, 64), (700, 2, 72)])
+def test_hip_model_follows_eager(T, B, H):
+    eager = model(vocab=500, hidden=H).cuda()
+    hip = model("hip", vocab=500, hidden=H).cuda()
+    hip.load_state_dict(eager.state_dict())
+    x, y = batch(T, B, 500, device="cuda")
+    out = []
+    for m in (eager, hip):
+        m.train()
+        states = m.state_init(B)
+        gen = torch.Generator().manual_seed(3)
+        for k, (h, c) in enumerate(states):
+            c.copy_(torch.randn(c.shape, generator=gen))
+        scores, states = m(x, states)
+        loss = F_ref.nll_loss(scores, y)
+        loss.backward()
+        out.append((scores, states, [p.grad for p in m.parameters()]))
+    (s0, st0, g0), (s1, st1, g1) = out
+    assert rel(s1, s0) < SCORES
+    for (_, c0), (_, c1) in zip(st0, st1):
+        assert rel(c1, c0) < SCORES
+    for (name, _), a, b in zip(eager.named_parameters(), g1, g0):
+        assert rel(a, b) < GRADS, name
+
+
+@GPU
+def test_hip_tokens_one_by_one():
+    m = model("hip", vocab=300, hidden=136).cuda().eval()
+    x, _ = batch(10, 5, 300, device="cuda")
+    with torch.no_grad():
+        whole, last = m(x, m.state_init(5))
+        want = [c.clone() for _, c in last]
+        whole = whole.clone().view(10, 5, -1)
+        states = m.state_init(5)
+        first = states[0][1]
+        for t in range(10):
+            s, states = m(x[t:t + 1], states)
+            # the same gates, each rounded to bf16; a state's bits may differ
+            # where the scan composes its steps in another order, and an h
+            # at a border of bf16 with it
+            assert rel(s, whole[t]) < 2.0 ** -9
+        assert not first.any()          # the caller's state is left alone
+    for (_, c), w in zip(states, want):
+        assert rel(c, w) < 2.0 ** -9
+
+
+@GPU
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("cell", ["glr", "lstm"])
+def test_hip_adamw_trains(cell, bits):
+    """The HIP step against the eager one on the same gradients, and the
+    shadows that the next forward reads."""
+    torch.manual_seed(0)
+    m = Model(203, 72, 2, 0.0, 0.1, engine="hip", cell=cell).cuda()
+    opt = AdamW(m.parameters(), bits=bits)
+    twin = [p.detach().cpu().clone().requires_grad_() for p in m.parameters()]
+    other = AdamW(twin, bits=bits)
+    m.train()
+    states = m.state_init(4)
+    for step in range(3):
+        x, y = batch(11, 4, 203, seed=step, device="cuda")
+        m.zero_grad(set_to_none=True)
+        states = m.detach(states)
+        scores, states = m(x, states)
+        trainer.nll_loss(scores, y).backward()
+        for p, q in zip(m.parameters(), twin):
+            q.grad = p.grad.cpu()
+        norm = trainer.adamw_step(m, opt, 1e-2, 0.5)
+        want = other.step(1e-2, 0.5)
+        assert abs(float(norm) - float(want)) <= 2.0 ** -22 * float(want)
+        for p, q in zip(m.parameters(), twin):
+            # lr times 30 half steps a step (tests/test_adamw.py); in 8 bits
+            # a draw next to its border may move a code, 1 / 8 of a value
+            off = (p.detach().cpu() - q).abs()
+            if bits == 32:
+                assert float(off.max()) < (step + 1) * 32 * 2.0 ** -24
+            else:
+                assert float((off > 1e-5).float().mean()) < 1e-4
+            with torch.no_grad():
+                q.copy_(p.cpu())
+    m._hip_model.check_aborts()
+    before = scores.detach().clone()
+    m._hip_model.invalidate_shadows()   # read the masters again
+    with torch.no_grad():
+        a, _ = m(x, m.state_init(4))
+        a = a.clone()
+        m._hip_model.refresh_shadows()
+        b, _ = m(x, m.state_init(4))
+    assert torch.equal(a, b) and not torch.equal(a, before)
+
+
+@GPU
+def test_hip_shadows_are_rewritten():
+    m = model("hip", vocab=101, hidden=40).cuda()
+    opt = AdamW(m.parameters())
+    x, y = batch(5, 3, 101, device="cuda")
+    scores, _ = m(x, m.state_init(3))
+    trainer.nll_loss(scores, y).backward()
+    trainer.adamw_step(m, opt, 1e-1, 1.0)
+    hm = m._hip_model
+    assert torch.equal(hm.emb_W, m.embed.W.detach().bfloat16())
+    assert torch.equal(hm.fc.W, m.fc.W.detach().bfloat16())
+    assert torch.equal(hm.fc.WT[:, :101], hm.fc.W.t())
+    for rt, layer in zip(hm.layers, m.rnns):
+        assert torch.equal(rt.Wx, layer.W_x.detach().bfloat16())
+        assert torch.equal(rt.WxT[:, :160], rt.Wx.t())
+
+
+@GPU
+@pytest.mark.parametrize("bits", [32, 8])
+def test_training_loop_runs(tmp_path, bits, capsys):
+    """trainer.train on the HIP engine, windows, epochs and a checkpoint."""
+    from zaremba_amd import data as zdata
+    trn, vld, tst, vocab = zdata.synthetic_init(
+        vocab_size=50, train_tokens=3000, valid_tokens=600, test_tokens=600,
+        seed=1)
+    sets = tuple(zdata.minibatch(d, 4, 10) for d in (trn, vld, tst))
+    m = model("hip", vocab=vocab, hidden=48, dropout=0.1).cuda()
+    opt = AdamW(m.parameters(), bits=bits)
+    path = str(tmp_path / "m.pt")
+    ppl = trainer.train(sets, m, 2, 1, 5e-3, 1.0, 5.0, 4, save_path=path,
+                        optimizer=opt)
+    assert ppl == ppl and ppl < 1e4
+    assert "Training is over." in capsys.readouterr().out
+    m2, payload = build_model_from_checkpoint(path, engine="hip")
+    m2.cuda()
+    opt2 = AdamW(m2.parameters(), bits=bits)
+    opt2.load_state_dict(payload["optimizer"])
+    assert int(opt2.step_count) == 2 * len(sets[0])
+    for a, b in zip(opt.exp_avgs, opt2.exp_avgs):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))

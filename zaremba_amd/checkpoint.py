@@ -10,6 +10,7 @@ framework's on-disk format: a single ``.pt`` file holding
     reference model.py:11,26-29,62-63) — fp32 master weights
   * ``model_args`` needed to rebuild the architecture
   * run metadata: epoch, lr, torch RNG state
+  * ``optimizer``, where AdamW trains: its ``state_dict``
 
 so ensemble training can parallelize across ranks and any subset of
 saved models can be re-loaded for averaged evaluation.
@@ -34,6 +35,7 @@ def save_checkpoint(path: str, model, epoch: int = 0, lr: float = 0.0,
             "dropout": model.dropout_p,
             "winit": model.winit,
             "lstm_type": model.lstm_type,
+            "cell": model.cell,
         },
         "epoch": epoch,
         "lr": lr,

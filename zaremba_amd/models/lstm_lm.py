@@ -16,7 +16,9 @@ MI355X-native specifics:
   * both --lstm_type values ("pytorch" and "custom") execute the same
     fused HIP cell — the reference's nn.LSTM fast path and its custom
     cell are one implementation here; parameter naming
-    always follows the custom convention (W_x/W_h/b_x/b_h per layer).
+    always follows the custom convention (W_x/W_h/b_x/b_h per layer),
+  * ``cell="glr"`` puts the gated linear recurrence in the LSTM's place: the
+    same gates without W_h, so that time is a scan (ops/glr.py).
 """
 
 from __future__ import annotations
@@ -69,6 +71,28 @@ class LSTM(nn.Module):
         return f"LSTM(input: {self.input_size}, hidden: {self.hidden_size})"
 
 
+class GLR(nn.Module):
+    """One layer of the gated linear recurrence: the LSTM cell without its
+    recurrent product (ops/glr.py). Gate order (i, f, o, n); states are
+    (h, c) as the LSTM's, of which only c is read."""
+
+    def __init__(self, input_size: int, hidden_size: int):
+        super().__init__()
+        self.input_size = input_size
+        self.hidden_size = hidden_size
+        self.W_x = nn.Parameter(torch.Tensor(4 * hidden_size, input_size))
+        self.b_x = nn.Parameter(torch.Tensor(4 * hidden_size))
+
+    def forward(self, x, states):
+        T, B = x.shape[:2]
+        gates = torch.addmm(self.b_x, x.reshape(T * B, -1), self.W_x.t())
+        out, c = F_ref.glr_layer(gates.view(T, B, -1), states[1])
+        return out, (out[-1], c)
+
+    def __repr__(self):
+        return f"GLR(input: {self.input_size}, hidden: {self.hidden_size})"
+
+
 class Linear(nn.Module):
     """Output projection; returns 2-D [T*B, V] scores (reference model.py:57-71)."""
 
@@ -89,12 +113,15 @@ class Linear(nn.Module):
 class Model(nn.Module):
     def __init__(self, vocab_size: int, hidden_size: int, layer_num: int,
                  dropout: float, winit: float, lstm_type: str = "custom",
-                 engine: str = "auto"):
+                 engine: str = "auto", cell: str = "lstm"):
         super().__init__()
         if lstm_type not in ("pytorch", "custom"):
             raise ValueError(f"unknown lstm_type {lstm_type!r}")
         if engine not in ("auto", "hip", "eager"):
             raise ValueError(f"unknown engine {engine!r}")
+        if cell not in ("lstm", "glr"):
+            raise ValueError(f"unknown cell {cell!r}")
+        self.cell = cell
         self.vocab_size = vocab_size
         self.hidden_size = hidden_size
         self.layer_num = layer_num
@@ -104,7 +131,8 @@ class Model(nn.Module):
         self.dropout_p = dropout
         self.embed = Embed(vocab_size, hidden_size)
         self.rnns = nn.ModuleList(
-            [LSTM(hidden_size, hidden_size) for _ in range(layer_num)]
+            [(LSTM if cell == "lstm" else GLR)(hidden_size, hidden_size)
+             for _ in range(layer_num)]
         )
         self.fc = Linear(hidden_size, vocab_size)
         self.dropout = nn.Dropout(p=dropout)

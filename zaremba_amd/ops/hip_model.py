@@ -22,7 +22,9 @@ from typing import Optional
 import torch
 
 from .. import _C  # noqa
-from .hip_ops import DropoutFn, EmbeddingFn, LinearFn, LstmLayerFn
+from .glr import glr_step
+from .hip_ops import (DropoutFn, EmbeddingFn, GlrLayerFn, LinearFn,
+                      LstmLayerFn)
 
 
 def _ks(k):
@@ -123,10 +125,18 @@ class _LayerRuntime:
         self.xT_buf = None   # persistent [Hin, TBp] transposed-x temp
         self.owner = None    # back-ref to the HipModel (side stream)
 
+    def shadows(self, layer):
+        return [(layer.W_x, self.Wx), (layer.W_h, self.Wh)]
+
     @torch.no_grad()
     def refresh(self, layer, e):
         self.Wx.copy_(layer.W_x)
         self.Wh.copy_(layer.W_h)
+        self.refresh_derived(layer, e)
+
+    @torch.no_grad()
+    def refresh_derived(self, layer, e):
+        """What follows from the shadows: transposes, packs, folded bias."""
         e.transpose_bf16(self.Wx, self.WxT)
         e.transpose_bf16(self.Wh, self.WhT)
         e.pack_gated_w(self.Wh, self.WhP, self.H, 4, self.H)
@@ -136,6 +146,52 @@ class _LayerRuntime:
     def ensure_ws(self, T, B, device, slack_ptrs=None):
         if self.ws is None or self.ws.T != T or self.ws.B != B:
             self.ws = _LayerWorkspace(T, B, self.H, device, slack_ptrs)
+        return self.ws
+
+
+class _GlrWorkspace:
+    def __init__(self, T: int, B: int, H: int, device, slack_ptrs=None):
+        bf = torch.bfloat16
+        self.T, self.B, self.H = T, B, H
+        self.gates = torch.zeros(T, B, 4 * H, dtype=bf, device=device)
+        self.h = torch.zeros(T, B, H, dtype=bf, device=device)
+        # the dx GEMM's A operand, which over-reads into the slack
+        self.dG = _slacked((T, B, 4 * H), bf, device, slack_ptrs)
+        self.TBp = _pad64(T * B)
+        self.dGT = torch.zeros(4 * H, self.TBp, dtype=bf, device=device)
+
+
+class _GlrRuntime:
+    """Shadows + workspace for one layer of the gated linear recurrence."""
+
+    def __init__(self, layer, device):
+        self.H = layer.hidden_size
+        self.Hin = layer.input_size
+        bf = torch.bfloat16
+        self.Wx = torch.empty_like(layer.W_x, dtype=bf, device=device)
+        self.H4p = _pad64(4 * self.H)  # see _LayerRuntime
+        self.WxT = torch.zeros(self.Hin, self.H4p, dtype=bf, device=device)
+        self.ws: Optional[_GlrWorkspace] = None
+        self.slack_ptrs = None
+        self.dx_part = None
+        self.xT_buf = None
+        self.owner = None
+
+    def shadows(self, layer):
+        return [(layer.W_x, self.Wx)]
+
+    @torch.no_grad()
+    def refresh(self, layer, e):
+        self.Wx.copy_(layer.W_x)
+        self.refresh_derived(layer, e)
+
+    @torch.no_grad()
+    def refresh_derived(self, layer, e):
+        e.transpose_bf16(self.Wx, self.WxT)
+
+    def ensure_ws(self, T, B, device, slack_ptrs=None):
+        if self.ws is None or self.ws.T != T or self.ws.B != B:
+            self.ws = _GlrWorkspace(T, B, self.H, device, slack_ptrs)
         return self.ws
 
 
@@ -188,7 +244,8 @@ class HipModel:
         # these may be the A operand of a k_pad GEMM (ext_bind.hip:gemm).
         self.slack_ptrs = set()
         self._slack_bufs = {}
-        self.layers = [_LayerRuntime(l, dev) for l in model.rnns]
+        runtime = _LayerRuntime if model.cell == "lstm" else _GlrRuntime
+        self.layers = [runtime(l, dev) for l in model.rnns]
         for rt in self.layers:
             rt.slack_ptrs = self.slack_ptrs
         self.fc = _FcRuntime(model.fc, dev)
@@ -259,6 +316,8 @@ class HipModel:
         GPU, but the step's outputs are then garbage). Called from the
         trainer's log steps, which synchronize anyway — failure detection
         at zero steady-state cost."""
+        if self.model.cell != "lstm":
+            return  # no such kernels
         for rt in self.layers:
             if rt.ws is not None and int(rt.ws.abort.item()) != 0:
                 raise RuntimeError(
@@ -285,7 +344,7 @@ class HipModel:
             self.refresh_shadows()
         m = self.model
         T, B = x.shape
-        if B > 32:
+        if B > 32 and m.cell == "lstm":
             # Every cell kernel (persistent, fused backward, per-step
             # fallback) tiles the batch into the 32-row MFMA pair;
             # larger per-GPU batches are out of contract — fail loudly
@@ -309,9 +368,12 @@ class HipModel:
         for i, (rt, layer) in enumerate(zip(self.layers, m.rnns)):
             rt.ensure_ws(T, B, self.device, self.slack_ptrs)
             h0, c0 = states[i]
-            out, hT, cT = LstmLayerFn.apply(cur, h0, c0, layer.W_x,
-                                            layer.W_h, layer.b_x, layer.b_h,
-                                            rt)
+            if m.cell == "glr":
+                out, hT, cT = self._glr_layer(cur, c0, layer, rt)
+            else:
+                out, hT, cT = LstmLayerFn.apply(cur, h0, c0, layer.W_x,
+                                                layer.W_h, layer.b_x,
+                                                layer.b_h, rt)
             new_states[i] = (hT, cT)
             cur = out
             if training and p > 0:
@@ -325,7 +387,59 @@ class HipModel:
             states[i] = new_states[i]
         return scores, states
 
+    def _glr_layer(self, x, c0, layer, rt):
+        if x.size(0) > 1 or torch.is_grad_enabled():
+            return GlrLayerFn.apply(x, c0, layer.W_x, layer.b_x, rt,
+                                    torch.is_grad_enabled())
+        # one token: the state is advanced in place, in a copy of the
+        # caller's
+        B, H = x.size(1), rt.H
+        gates = rt.ws.gates.view(B, 4 * H)
+        self.e.gemm(x.reshape(B, -1).contiguous(), rt.Wx, gates, layer.b_x,
+                    False, False)
+        c = c0.to(torch.float32, copy=True)
+        h = glr_step(gates, c)
+        return h.view(1, B, H), h, c
+
     # ------------------------------------------------------------------
+    def _shadow_of(self):
+        m = self.model
+        shadow_of = {id(m.embed.W): self.emb_W, id(m.fc.W): self.fc.W}
+        for rt, layer in zip(self.layers, m.rnns):
+            for p, sh in rt.shadows(layer):
+                shadow_of[id(p)] = sh
+        return shadow_of
+
+    def _refresh_derived(self):
+        """After an update that rewrote the shadows."""
+        for rt, layer in zip(self.layers, self.model.rnns):
+            rt.refresh_derived(layer, self.e)
+        self.e.transpose_bf16(self.fc.W, self.fc.WT)
+
+    def _join_side_stream(self, params):
+        """The side-stream weight-grad work, before any grad is read."""
+        cur = torch.cuda.current_stream()
+        for ev in self.side_events:
+            cur.wait_event(ev)
+        self.side_events.clear()
+        if self.side_stream is not None:
+            # caching-allocator cross-stream rule: grads allocated on the
+            # side stream are consumed here on the main stream
+            for p in params:
+                p.grad.record_stream(cur)
+
+    @torch.no_grad()
+    def clip_and_adamw(self, opt, lr: float, max_norm: float,
+                       grad_scale: float = 1.0):
+        """Global grad-norm clip + AdamW (ops/adamw.py), rewriting the bf16
+        shadows in the same pass. Returns the pre-clip grad norm as a 0-d
+        device tensor."""
+        self._join_side_stream([p for p in self.model.parameters()
+                                if p.grad is not None])
+        norm = opt.step(lr, max_norm, grad_scale, self._shadow_of())
+        self._refresh_derived()
+        return norm
+
     @torch.no_grad()
     def clip_and_sgd(self, lr: float, max_norm: float,
                      grad_scale: float = 1.0):
@@ -338,23 +452,10 @@ class HipModel:
         """
         m = self.model
         e = self.e
-        # join the side-stream weight-grad work before any grad is read
-        cur = torch.cuda.current_stream()
-        if self.side_events:
-            for ev in self.side_events:
-                cur.wait_event(ev)
-            self.side_events.clear()
-        self.norm2.zero_()
         params = [p for p in m.parameters() if p.grad is not None]
-        if self.side_stream is not None:
-            # caching-allocator cross-stream rule: grads allocated on the
-            # side stream are consumed here on the main stream
-            for p in params:
-                p.grad.record_stream(cur)
-        shadow_of = {id(m.embed.W): self.emb_W, id(m.fc.W): self.fc.W}
-        for rt, layer in zip(self.layers, m.rnns):
-            shadow_of[id(layer.W_x)] = rt.Wx
-            shadow_of[id(layer.W_h)] = rt.Wh
+        self._join_side_stream(params)
+        self.norm2.zero_()
+        shadow_of = self._shadow_of()
         # Chunked multi-tensor descriptors: one norm launch + one update
         # launch for all params. Grad tensors are fresh per step, but the
         # caching allocator cycles through a small set of addresses, so
@@ -392,12 +493,6 @@ class HipModel:
             cache[key] = descs
         e.norm2_mt(descs[0], self.norm2)
         e.sgd_mt(descs[1], self.norm2, max_norm, lr, grad_scale)
-        # refresh the derived shadows (transposes + packs + folded biases)
-        for rt, layer in zip(self.layers, m.rnns):
-            e.transpose_bf16(rt.Wx, rt.WxT)
-            e.transpose_bf16(rt.Wh, rt.WhT)
-            e.pack_gated_w(rt.Wh, rt.WhP, rt.H, 4, rt.H)
-            e.pack_gated_w(rt.WhT, rt.WhTP, rt.H, 1, 4 * rt.H)
-            torch.add(layer.b_x, layer.b_h, out=rt.bias_sum)
-        e.transpose_bf16(self.fc.W, self.fc.WT)
+        # the derived shadows (transposes + packs + folded biases)
+        self._refresh_derived()
         return (self.norm2.sqrt() * grad_scale).reshape(())

@@ -309,3 +309,64 @@ class LstmLayerFn(torch.autograd.Function):
                    rt.H4p if rt.H4p != 4 * H else 0)
         return (dx.view(T, B, Hin), None, None, dWx, dWh, db, db2,
                 None)
+
+
+class GlrLayerFn(torch.autograd.Function):
+    """One layer of the gated linear recurrence: the gate GEMM of the whole
+    window, then the scan; backward the scan's gradient, then the batched
+    dW / dx GEMMs as in LstmLayerFn. Workspaces are the layer runtime's (see
+    the aliasing contract above)."""
+
+    @staticmethod
+    def forward(ctx, x, c0, Wx_m, bx_m, rt, training):
+        T, B, Hin = x.shape
+        x2 = x.contiguous()
+        e = ext()
+        ws = rt.ws
+        e.gemm(x2.view(T * B, Hin), rt.Wx, ws.gates.view(T * B, 4 * rt.H),
+               bx_m, False, False)
+        c0 = c0.to(torch.float32)
+        _, cT, marks = e.glr_forward(ws.gates, c0, None, training, ws.h)
+        out, hT = ws.h[:], ws.h[T - 1]  # views: ws.h itself joins no graph
+        ctx.save_for_backward(x2, c0, marks)
+        ctx.rt = rt
+        ctx.mark_non_differentiable(hT, cT)
+        return out, hT, cT
+
+    @staticmethod
+    def backward(ctx, dY, dhT, dcT):
+        x2, c0, marks = ctx.saved_tensors
+        rt = ctx.rt
+        ws = rt.ws
+        e = ext()
+        T, B, Hin = x2.shape
+        TB, H = T * B, rt.H
+        e.glr_backward(dY.to(torch.bfloat16), None, ws.gates, c0, marks,
+                       None, ws.dG)
+        dG2 = ws.dG.view(TB, 4 * H)
+        # dW_x = dG^T @ x over transposed, zero-padded temps (LstmLayerFn)
+        e.transpose_bf16(dG2, ws.dGT)
+        if rt.xT_buf is None or rt.xT_buf.shape != (Hin, ws.TBp):
+            rt.xT_buf = torch.zeros(Hin, ws.TBp, dtype=torch.bfloat16,
+                                    device=x2.device)
+        e.transpose_bf16(x2.view(TB, Hin), rt.xT_buf)
+        dWx = torch.empty(4 * H, Hin, dtype=torch.float32, device=x2.device)
+        e.gemm(ws.dGT, rt.xT_buf, dWx, None, False, False)
+        db = torch.zeros(4 * H, dtype=torch.float32, device=x2.device)
+        e.colsum_bf16(dG2, db)
+        dx = torch.empty(TB, Hin, dtype=torch.bfloat16, device=x2.device)
+        if rt.H4p >= 128:
+            if rt.dx_part is None or rt.dx_part[0].shape != (TB, Hin):
+                rt.dx_part = (
+                    torch.empty(TB, Hin, dtype=torch.float32,
+                                device=x2.device),
+                    torch.empty(3, TB, Hin, dtype=torch.float32,
+                                device=x2.device))
+            p1, pex = rt.dx_part
+            nz = e.gemm_splitk(dG2, rt.WxT, p1, pex, None,
+                               rt.H4p if rt.H4p != 4 * H else 0)
+            e.addn_f32_bf16(p1, pex, dx, nz)
+        else:
+            e.gemm(dG2, rt.WxT, dx, None, False, False,
+                   rt.H4p if rt.H4p != 4 * H else 0)
+        return dx.view(T, B, Hin), None, dWx, db, None, None

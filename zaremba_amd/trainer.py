@@ -101,6 +101,17 @@ def sgd_step(model, lr: float, max_norm: float, grad_scale: float = 1.0):
     return F_ref.clip_grad_and_sgd_(list(model.parameters()), max_norm, lr)
 
 
+def adamw_step(model, opt, lr: float, max_norm: float,
+               grad_scale: float = 1.0):
+    """Grad clip + AdamW with the states of ``opt`` (ops.adamw.AdamW over
+    ``model.parameters()``), dispatched as sgd_step is. Returns the pre-clip
+    grad norm as a 0-d tensor."""
+    dev = next(model.parameters()).device
+    if dev.type == "cuda" and model._resolve_engine(dev) == "hip":
+        return model.hip().clip_and_adamw(opt, lr, max_norm, grad_scale)
+    return opt.step(lr, max_norm, grad_scale)
+
+
 def train(
     data: Tuple[List, List, List],
     model,
@@ -117,13 +128,16 @@ def train(
     start_epoch: int = 0,
     dp=None,
     is_rank0: bool = True,
+    optimizer=None,
 ):
     """The training loop (reference main.py:97-133 / ensemble.py:128-164).
 
     ``log_every=None`` -> the reference's len(trn)//10 cadence; ensemble
     mode passes 800. ``dp`` is an optional parallel.Bucketer handling
     gradient all-reduce overlap; ``start_epoch``/``save_path`` implement
-    resume (additive; the reference has no checkpointing).
+    resume (additive; the reference has no checkpointing). ``optimizer``:
+    an ops.adamw.AdamW in place of the reference's manual SGD; its states
+    are saved with the model.
     """
     trn, vld, tst = data
     tic = timeit.default_timer()
@@ -169,7 +183,8 @@ def train(
             # "global batch 160" semantics of BASELINE config 4. No
             # averaging (grad_scale stays 1).
             with trace_range("clip_sgd"):
-                norm = sgd_step(model, lr, max_norm)
+                norm = (sgd_step(model, lr, max_norm) if optimizer is None
+                        else adamw_step(model, optimizer, lr, max_norm))
             if i % cadence == 0:
                 if model._hip_model is not None:
                     model._hip_model.check_aborts()
@@ -206,7 +221,10 @@ def train(
                       "lr": lr})
             if save_path:
                 from .checkpoint import save_checkpoint
-                save_checkpoint(save_path, model, epoch=epoch + 1, lr=lr)
+                save_checkpoint(
+                    save_path, model, epoch=epoch + 1, lr=lr,
+                    extra=None if optimizer is None else
+                    {"optimizer": optimizer.state_dict()})
     tst_perp = perplexity(tst, model, batch_size)
     if model._hip_model is not None:
         model._hip_model.check_aborts()
