@@ -74,14 +74,13 @@ DEV_INLINE void store_some(T* p, const Quad<T>& x, int n) {
     if (e < n) p[e] = x.v[e];
 }
 
-// The tensor that chunk `c` of a launch belongs to.
+// The tensor that chunk `c` of a launch belongs to: a lane for each, so that
+// it costs one round trip to the arguments.
 DEV_INLINE int tensor_of(const int* begin, int count, int c) {
-  int lo = 0, hi = count;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (begin[mid] <= c) lo = mid; else hi = mid;
-  }
-  return lo;
+  static_assert(ADAMW_TENSORS <= 64);
+  const int lane = lane_id();
+  const int b = begin[lane < count ? lane : 0];
+  return __popcll(__ballot(lane < count && b <= c)) - 1;
 }
 
 // How many of a tensor's n values chunk number `c` has. The comparison is in 32
@@ -102,9 +101,11 @@ DEV_INLINE double block_sum(double x, double* lds) {
 
 template <typename G>
 __global__ __launch_bounds__(THREADS) void adamw_norm_kernel(
-    AdamwTensors a, AdamwScalars s, int first, AdamwWork w) {
+    AdamwTensors a, AdamwScalars s, int first, int blocks, AdamwWork w) {
   __shared__ double lds[WAVES];
-  if (first + blockIdx.x == 0 && threadIdx.x == 0) {
+  if ((int)blockIdx.x == blocks) {
+    // one block more, in the first launch, for the step's own values
+    if (threadIdx.x) return;
     const int64_t t = *s.step + 1;
     *s.step = t;
     double p1 = 1, p2 = 1, x1 = s.beta1, x2 = s.beta2;
@@ -116,37 +117,36 @@ __global__ __launch_bounds__(THREADS) void adamw_norm_kernel(
     w.values->rate = (float)(s.lr / (1 - p1));
     w.values->root = (float)(1 / __builtin_sqrt(1 - p2));
     w.values->step = (unsigned)t;
+    return;
   }
-  if (!s.clip) return;
   double sum = 0;
-  for (int c = blockIdx.x; c < a.norm_begin[a.count]; c += gridDim.x) {
+  for (int c = blockIdx.x; c < a.norm_begin[a.count]; c += blocks) {
     const int k = tensor_of(a.norm_begin, a.count, c);
     const int rel = c - a.norm_begin[k];
     const int n = chunk_length(a.t[k].n, rel, ADAMW_NORM_CHUNK);
     const G* g =
         static_cast<const G*>(a.t[k].g) + (int64_t)rel * ADAMW_NORM_CHUNK;
+    // A chunk that ends early reads its last four again, and leaves them out.
     constexpr int R = ADAMW_NORM_CHUNK / THREADS / 4;
-    if (n == ADAMW_NORM_CHUNK) {
+    const int quads = n / 4;
+    if (quads > 0) {
       Quad<G> x[R];
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        x[r] = load4(g + (r * THREADS + threadIdx.x) * 4);
+        x[r] = load4(g + min(r * THREADS + (int)threadIdx.x, quads - 1) * 4);
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r) {
+        const bool in = r * THREADS + (int)threadIdx.x < quads;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const double y = (double)(float)x[r].v[e];
+          const double y = in ? (double)(float)x[r].v[e] : 0.;
           sum = __builtin_fma(y, y, sum);  // y * y is exact
         }
-    } else {
-      for (int i = threadIdx.x * 4; i < n; i += THREADS * 4) {
-        const Quad<G> x = load_some(g + i, n - i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const double y = (double)(float)x.v[e];
-          sum = __builtin_fma(y, y, sum);
-        }
       }
+    }
+    if ((int)threadIdx.x < n % 4) {
+      const double y = (double)(float)g[quads * 4 + threadIdx.x];
+      sum = __builtin_fma(y, y, sum);
     }
   }
   sum = block_sum(sum, lds);
@@ -348,10 +348,11 @@ struct Block {
                                           true);
       __builtin_memcpy(&m, &c, 4);
       const unsigned hashed = x.hashed + i * HASH_INDEX;
+      unsigned codes = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        v.v[e] =
-            (uint8_t)draw_e4m3(r1.v[e] * ir, hashed + e * HASH_INDEX);
+        codes |= draw_e4m3(r1.v[e] * ir, hashed + e * HASH_INDEX) << 8 * e;
+      __builtin_memcpy(&v, &codes, 4);
     }
     if (WHOLE) {
       store4(x.p + i, p);
@@ -404,10 +405,9 @@ __global__ __launch_bounds__(THREADS) void adamw_update_kernel(
     for (int r = 0; r < AHEAD; ++r) {
       const int i = q + r * STRIDE;
       if (i >= whole) break;
-      Block<G, BITS8> now = b[r];
+      b[r].template update<true>(x, i, 4, s, coef, rate, root);
       if (i + AHEAD * STRIDE < whole)
         b[r].template load<true>(x, i + AHEAD * STRIDE, 4);
-      now.template update<true>(x, i, 4, s, coef, rate, root);
     }
   }
   // what is left of the tensor behind its last whole 256
@@ -432,8 +432,9 @@ void launch_adamw_norm(const AdamwTensors& a, const AdamwScalars& s,
                        const AdamwWork& w, hipStream_t stream) {
   auto kernel =
       bf16_grads ? adamw_norm_kernel<bf16> : adamw_norm_kernel<float>;
-  hipLaunchKernelGGL(kernel, dim3(s.clip ? blocks : 1), dim3(THREADS), 0,
-                     stream, a, s, first, w);
+  if (!s.clip) blocks = 0;
+  hipLaunchKernelGGL(kernel, dim3(blocks + (first == 0)), dim3(THREADS), 0,
+                     stream, a, s, first, blocks, w);
 }
 
 void launch_adamw_update(const AdamwTensors& a, const AdamwScalars& s,

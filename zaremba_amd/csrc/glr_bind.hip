@@ -228,6 +228,10 @@ std::tuple<Tensor, Tensor> glr_backward(
 
 Tensor glr_step(const Tensor& gates_in, const Tensor& c) {
   const char* op = "glr_step";
+  TORCH_CHECK(!at::GradMode::is_enabled() ||
+              !(gates_in.requires_grad() || c.requires_grad()),
+              op, ": has no backward pass; call it under torch.no_grad(), or "
+              "use glr()");
   check_gates(gates_in, 2, op);
   const GlrType type = glr_type(gates_in, op);
   c10::DeviceGuard guard(gates_in.device());

@@ -111,11 +111,11 @@ def glr_step(gates, c):
     """One token: ``h`` [B, H] from ``gates`` [B, 4H]; the state ``c``
     (float32 [B, H], rows may be apart) is advanced in place. Has no
     backward pass: call it under ``torch.no_grad()``."""
+    if not _eager(gates):
+        return _C.ext().glr_step(gates, c)
     if torch.is_grad_enabled() and (gates.requires_grad or c.requires_grad):
         raise RuntimeError("glr_step: has no backward pass; call it under "
                            "torch.no_grad(), or use glr()")
-    if not _eager(gates):
-        return _C.ext().glr_step(gates, c)
     _check_eager("glr_step", gates, 2, c=c)
     h, new = F_ref.glr_step(gates, c)
     c.copy_(new)
