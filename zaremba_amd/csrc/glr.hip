@@ -14,18 +14,17 @@
 // are zero whatever stands there: such a step is (x, y) = (1, 0) by selects.
 //
 // Steps compose: c -> A c + C with A = prod x and C the state that the steps
-// reach from zero. A block takes 64 channels and walks the time axis in tiles
-// of W * K steps, wave w holding K of them in registers: each wave finds its
-// (A, C), the waves exchange them through LDS, and each then runs its own
-// steps from the state that the waves before it leave. Data is read once,
-// 4 K loads of a wave are in flight together, and a step waits for no other
-// but through one exchange a tile (two in the backward pass).
+// reach from zero. A block takes 64 channels and a tile of W * K steps, wave w
+// holding K of them in registers: each wave finds its (A, C), the waves
+// exchange them through LDS, and each then runs its own steps from the state
+// that the waves before it leave. Data is read once, 4 K loads of a wave are
+// in flight together, and a step waits for no other but through one exchange
+// (two in the backward pass). Longer windows are many such blocks (see below).
 //
 // A lane has one channel, so that rows may have any length and alignment. Two
 // channels a lane, with loads twice as wide, measured 264 to 290 us against
-// 260 forward and 521 to 576 against 533 backward at 65536 x 1 x 1500: the
-// registers of twice the steps leave half the waves.
-
+// 260 forward and 521 to 576 against 533 backward at 65536 x 1 x 1500 bf16:
+// the registers of twice the steps leave half the waves.
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
@@ -149,51 +148,73 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
   return c;
 }
 
-// Where the channels make too few blocks for 256 CUs, the time axis is cut
-// into chunks of one tile, a block each, and the state is handed from chunk
-// to chunk while all of them are in flight. Slot r, the r-th chunk in the
-// order of the scan, has a word for each channel. It first publishes its
-// (A, C) there and, once it knows the state before it, the state behind it
-// instead, marked by A = -1. A wave looks back over the slots before its own,
-// DEPTH of them at a time, and composes their pairs until it meets a state.
-// A word says by itself whether it is there (all ones: not yet; no word that
-// is written is), so that no order between stores is needed, and words go
-// past the L2s, which do not see each other's writes.
+// A window of more than one tile is a block for each tile, all in flight at
+// once, that hand the state on. Slot r, the r-th tile in the order of the
+// scan, has a word for each channel. It first publishes its (A, C) there and,
+// once it knows the state before it, the state behind it instead, marked by
+// A = -1. A wave looks back over the slots before its own, DEPTH of them at a
+// time, and composes their pairs until it meets a state. A word says by itself
+// whether it is there (all ones: not yet; no word that is written is), so that
+// no order between stores is needed, and words go past the L2s, which do not
+// see each other's writes.
 //
 // Blocks take their slots from a counter as they start. A block therefore
 // waits only for blocks that run already, and these only for earlier ones:
 // every wait ends, whatever the number of blocks that fit the chip. Polls are
 // bounded all the same; behind a bound that is reached the state is NaN.
 //
-// At T = 65536, B = 1, H = 1500, bf16 a chain takes 255 us forward (983 MB,
-// 3.9 TB/s of the 5.2 that a copy reaches) and 528 us backward (1770 MB, 3.4
-// TB/s); vector instructions take half of either, and without looking back at
-// all it is 248 and 516. Finding the (A, C) of long chunks in a launch of its
-// own, which reads three gates twice, took 360 and 680.
+// From SHARED_FROM groups of 64 channels on each of the 8 XCDs has a counter
+// and a share of the groups, neighbours side by side: rows of 64 values are
+// seldom whole cache lines, and the other halves are then met in the same L2.
+// Measured in us, forward / backward, one counter against eight: 375 groups x
+// 1024 steps 77 / 153 against 64 / 120, 94 x 4096 76 / 148 against 66 / 126;
+// but 23.4 x 65536 265 / 552 against 274 / 575, where an XCD has 3 groups.
+//
+// At T = 65536, B = 1, H = 1500, bf16 this takes 259 us forward (983 MB, 3.8
+// TB/s of the 5.2 that a copy reaches) and 566 backward (1770 MB, 3.1 TB/s);
+// with rows of whole lines, H = 1472, 203 (4.8 TB/s) and 373 (4.7). Vector
+// instructions take half of either. Before, finding the (A, C) of long chunks
+// in a launch of its own, which reads three gates twice, took 360 and 680, and
+// a block that loops over its tiles 2380 and 4500.
 constexpr unsigned ABSENT = 0xffffffffu;
 constexpr int MOST_POLLS = 1 << 22;
-constexpr int COUNTER_WORDS = GLR_COUNTER_WORDS;  // before the slots
+constexpr int COUNTERS_LOG2 = 3;   // one counter, or one for each XCD
+constexpr int COUNTER_APART = 16;  // words: 128 bytes
+constexpr int COUNTER_WORDS = COUNTER_APART << COUNTERS_LOG2;  // go first
 constexpr int DEPTH = 4;
 
 DEV_INLINE unsigned to_bits(float x) {  // any NaN but ABSENT
   return x == x ? __builtin_bit_cast(unsigned, x) : 0x7fc00000u;
 }
 
+// A block's place in the time order, and its 64 channels.
+struct Slot {
+  int order, group;
+};
+
 struct Chain {
-  unsigned* counter;
   uint64_t* words;  // [chunks, B * H]: A above C
   int64_t BH;
 
   DEV_INLINE Chain(const GlrArgs& a)
-      : counter(reinterpret_cast<unsigned*>(a.work)),
-        words(a.work + COUNTER_WORDS), BH((int64_t)a.B * a.H) {}
+      : words(a.work + COUNTER_WORDS), BH((int64_t)a.B * a.H) {}
 
-  DEV_INLINE int take_slot(int* lds) const {
+  // Counter x deals out the slots of its own share of the groups.
+  static DEV_INLINE Slot take_slot(const GlrArgs& a, int* lds) {
+    const int x = blockIdx.x & ((1 << a.counters_log2) - 1);
     if (threadIdx.x == 0)
-      *lds = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
-                                         __HIP_MEMORY_SCOPE_AGENT);
+      *lds = (int)__hip_atomic_fetch_add(
+          reinterpret_cast<unsigned*>(a.work + x * COUNTER_APART), 1u,
+          __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int first = a.groups * x >> a.counters_log2;
+    const int n = (a.groups * (x + 1) >> a.counters_log2) - first;
     __syncthreads();
-    return __builtin_amdgcn_readfirstlane(*lds);
+    const int k = __builtin_amdgcn_readfirstlane(*lds);
+    // a share may be smaller than the largest: order a.chunks is none
+    Slot s;
+    s.order = n ? min(k / n, a.chunks) : a.chunks;
+    s.group = first + (n ? k % n : 0);
+    return s;
   }
 
   DEV_INLINE void publish(int slot, const Channel& ch, float A,
@@ -267,179 +288,166 @@ __global__ void glr_reset_kernel(uint4* work, int64_t n) {
                                     : uint4{ABSENT, ABSENT, ABSENT, ABSENT};
 }
 
-// W: waves of a block, in a chain and at most otherwise.
+// W: waves of a block, in a chain; at most, where one tile is the window.
 template <typename E, int K, int W, bool CHAIN>
 __global__ __launch_bounds__(64 * W) void glr_fwd_kernel(GlrArgs a) {
-  __shared__ Pair lds[2][W][64];
-  __shared__ float handed[CHAIN ? 64 : 1];
+  static_assert(GLR_MARK % K == 0);  // a mark is the start of a wave's steps
+  __shared__ Pair lds[W][64];
+  __shared__ float handed[64];
   __shared__ int taken;
   const int waves = CHAIN ? W : blockDim.x / 64, lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
-  const int span = waves * K;
-  const int slot = CHAIN ? Chain(a).take_slot(&taken) : blockIdx.x;
-  const int chunk = CHAIN ? slot / a.groups : 0;
-  const Channel ch(a, slot - chunk * a.groups);
+  const Slot slot =
+      CHAIN ? Chain::take_slot(a, &taken) : Slot{0, (int)blockIdx.x};
+  if (CHAIN && slot.order >= a.chunks) return;
+  const Channel ch(a, slot.group);
   const E* g0 = static_cast<const E*>(a.gates) + ch.first * a.gates_b;
-  const unsigned g_off = ch.offset<E>(a.gates_b);
   E* h0 = static_cast<E*>(a.h) + ch.first * a.h_b;
   const unsigned h_off = ch.offset<E>(a.h_b);
-  const int begin = chunk * span;
-  const int end = CHAIN ? min(begin + span, a.T) : a.T;
+  const int t0 = (slot.order * waves + w) * K;
 
   Gates<E, K> g;
-  g.load(a, g0, g_off, begin + w * K);
-  float c = !CHAIN && a.c0 ? a.c0[ch.state] : 0.f;
-  for (int tile = begin, side = 0; tile < end; tile += span, side ^= 1) {
-    const int t0 = tile + w * K;
-    g.mask(t0, ch.n_live);
-    float x[K], y[K], A = 1.f, C = 0.f;
-    E o[K];
+  g.load(a, g0, ch.offset<E>(a.gates_b), t0);
+  g.mask(t0, ch.n_live);
+  float x[K], y[K], A = 1.f, C = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      o[k] = g.o[k];
-      x[k] = sigmoid_f((float)g.f[k]);
-      y[k] = sigmoid_tanh((float)g.i[k], (float)g.n[k]);
-      C = x[k] * C + y[k];
-      A *= x[k];
-    }
-    if (!CHAIN && tile + span < end) g.load(a, g0, g_off, t0 + span);
-    lds[side][w][lane] = {A, C};
-    __syncthreads();
-    if (CHAIN) {
-      if (w == 0)
-#pragma unroll
-        for (int q = 1; q < W; ++q) {
-          const Pair p = lds[0][q][lane];
-          C = p.A * C + p.C;
-          A *= p.A;
-        }
-      c = Chain(a).hand_on(chunk, ch, A, C, a.c0, handed,
-                           end == a.T ? a.cT : nullptr, w);
-    }
-    float now = c = compose(c, lds[side], 0, w);
-    if (a.marks && t0 % GLR_MARK == 0 && t0 < end && ch.live)
-      a.marks[(int64_t)(t0 / GLR_MARK) * a.B * a.H + ch.state] = now;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int t = t0 + k;
-      now = x[k] * now + y[k];
-      const float h = sigmoid_tanh((float)o[k], now);
-      if (t < end && ch.live)
-        at(h0 + t * a.h_t, h_off) = t < ch.n_live ? (E)h : (E)0.f;
-    }
-    if (!CHAIN) c = compose(c, lds[side], w, waves);
+  for (int k = 0; k < K; ++k) {
+    x[k] = sigmoid_f((float)g.f[k]);
+    y[k] = sigmoid_tanh((float)g.i[k], (float)g.n[k]);
+    C = x[k] * C + y[k];
+    A *= x[k];
   }
-  if (!CHAIN && w == 0 && ch.live) a.cT[ch.state] = c;
+  lds[w][lane] = {A, C};
+  __syncthreads();
+  float c;
+  if (CHAIN) {
+    if (w == 0)
+#pragma unroll
+      for (int q = 1; q < W; ++q) {
+        const Pair p = lds[q][lane];
+        C = p.A * C + p.C;
+        A *= p.A;
+      }
+    c = Chain(a).hand_on(slot.order, ch, A, C, a.c0, handed,
+                         slot.order == a.chunks - 1 ? a.cT : nullptr, w);
+  } else {
+    c = a.c0 ? a.c0[ch.state] : 0.f;
+  }
+  c = compose(c, lds, 0, w);
+  if (a.marks && t0 % GLR_MARK == 0 && t0 < a.T && ch.live)
+    a.marks[(int64_t)(t0 / GLR_MARK) * a.B * a.H + ch.state] = c;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int t = t0 + k;
+    c = x[k] * c + y[k];
+    const float h = sigmoid_tanh((float)g.o[k], c);
+    if (t < a.T && ch.live)
+      at(h0 + t * a.h_t, h_off) = t < ch.n_live ? (E)h : (E)0.f;
+  }
+  // steps past T keep the state
+  if (!CHAIN && w == waves - 1 && ch.live) a.cT[ch.state] = c;
 }
 
-// Tiles begin at marks and are walked from the last.
+// Tiles begin at marks; in a chain the first slot has the last of them.
 template <typename E, int K, int W, bool CHAIN>
 __global__ __launch_bounds__(64 * W) void glr_bwd_kernel(GlrArgs a) {
   static_assert(K * W % GLR_MARK == 0);
-  __shared__ Pair lds[2][W][64];   // (A, C) of the states
-  __shared__ Pair back[2][W][64];  // (A, D) of their gradients, last first
-  __shared__ float handed[CHAIN ? 64 : 1];
+  __shared__ Pair lds[W][64];   // (A, C) of the states
+  __shared__ Pair back[W][64];  // (A, D) of their gradients, last wave first
+  __shared__ float handed[64];
   __shared__ int taken;
   const int waves = CHAIN ? W : blockDim.x / 64, lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
   const int rw = waves - 1 - w;
-  const int span = waves * K;
-  const int slot = CHAIN ? Chain(a).take_slot(&taken) : blockIdx.x;
-  const int order = CHAIN ? slot / a.groups : 0;
-  const Channel ch(a, slot - order * a.groups);
+  const Slot slot =
+      CHAIN ? Chain::take_slot(a, &taken) : Slot{0, (int)blockIdx.x};
+  if (CHAIN && slot.order >= a.chunks) return;
+  const Channel ch(a, slot.group);
   const E* g0 = static_cast<const E*>(a.gates) + ch.first * a.gates_b;
-  const unsigned g_off = ch.offset<E>(a.gates_b);
   const E* dh0 = static_cast<const E*>(a.dh) + ch.first * a.dh_b;
   const unsigned dh_off = ch.offset<E>(a.dh_b);
   E* d0 = static_cast<E*>(a.dgates) + ch.first * a.dgates_b;
   const unsigned d_off = ch.offset<E>(a.dgates_b);
-  const int begin = CHAIN ? (a.chunks - 1 - order) * span : 0;
-  const int end = CHAIN ? min(begin + span, a.T) : a.T;
+  const int begin = CHAIN ? (a.chunks - 1 - slot.order) * W * K : 0;
+  const int t0 = begin + w * K, stop = ch.n_live;
 
-  float carry = !CHAIN && a.dcT ? a.dcT[ch.state] : 0.f;
-  int side = 0;
-  for (int tile = begin + (end - 1 - begin) / span * span; tile >= begin;
-       tile -= span, side ^= 1) {
-    const int t0 = tile + w * K;
-    Gates<E, K> g;
-    g.load(a, g0, g_off, t0);
-    E dh[K];
+  Gates<E, K> g;
+  g.load(a, g0, ch.offset<E>(a.gates_b), t0);
+  E dh[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      dh[k] = at(dh0 + (int64_t)min(t0 + k, a.T - 1) * a.dh_t, dh_off);
-    float c = a.marks[(int64_t)(tile / GLR_MARK) * a.B * a.H + ch.state];
-
-    const int stop = ch.n_live;
-    g.mask(t0, stop);
-    if (!__all(t0 + K <= stop)) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        g.o[k] = t0 + k < stop ? g.o[k] : (E)0.f;
-        dh[k] = t0 + k < stop ? dh[k] : (E)0.f;
-      }
-    }
-    float i[K], f[K], n[K], A = 1.f, C = 0.f;
+  for (int k = 0; k < K; ++k)
+    dh[k] = at(dh0 + (int64_t)min(t0 + k, a.T - 1) * a.dh_t, dh_off);
+  float c = a.marks[(int64_t)(begin / GLR_MARK) * a.B * a.H + ch.state];
+  g.mask(t0, stop);
+  if (!__all(t0 + K <= stop)) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      i[k] = sigmoid_f((float)g.i[k]);
-      f[k] = sigmoid_f((float)g.f[k]);
-      n[k] = tanh_f((float)g.n[k]);
-      C = f[k] * C + i[k] * n[k];
-      A *= f[k];
+      g.o[k] = t0 + k < stop ? g.o[k] : (E)0.f;
+      dh[k] = t0 + k < stop ? dh[k] : (E)0.f;
     }
-    lds[side][w][lane] = {A, C};
-    __syncthreads();
-    c = compose(c, lds[side], 0, w);
-    // Forward again through the own steps; u is what a step adds to g, and
-    // D what the steps hand back from a gradient of zero behind them. The
-    // output gate's gradient needs no more and is written at once.
-    float before[K], u[K], D = 0.f;
+  }
+  float i[K], f[K], n[K], A = 1.f, C = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int t = t0 + k;
-      before[k] = c;
-      c = f[k] * c + i[k] * n[k];
-      const float tc = tanh_f(c);
-      const float o = sigmoid_f((float)g.o[k]);
-      const float od = o * (float)dh[k];
-      u[k] = od * (1.f - tc * tc);
-      if (t < end && ch.live)
-        at(d0 + t * a.dgates_t + 2 * (int64_t)a.H, d_off) =
-            t < stop ? (E)(od * tc * (1.f - o)) : (E)0.f;
-    }
+  for (int k = 0; k < K; ++k) {
+    i[k] = sigmoid_f((float)g.i[k]);
+    f[k] = sigmoid_f((float)g.f[k]);
+    n[k] = tanh_f((float)g.n[k]);
+    C = f[k] * C + i[k] * n[k];
+    A *= f[k];
+  }
+  lds[w][lane] = {A, C};
+  __syncthreads();
+  c = compose(c, lds, 0, w);
+  // Forward again through the own steps; u is what a step adds to g, and D
+  // what the steps hand back from a gradient of zero behind them. The output
+  // gate's gradient needs no more and is written at once.
+  float before[K], u[K], D = 0.f;
 #pragma unroll
-    for (int k = K - 1; k >= 0; --k) D = f[k] * (D + u[k]);
-    back[side][rw][lane] = {A, D};
-    __syncthreads();
-    if (CHAIN) {
-      float whole = 1.f, sum = 0.f;
-      if (w == 0)
+  for (int k = 0; k < K; ++k) {
+    const int t = t0 + k;
+    before[k] = c;
+    c = f[k] * c + i[k] * n[k];
+    const float tc = tanh_f(c);
+    const float o = sigmoid_f((float)g.o[k]);
+    const float od = o * (float)dh[k];
+    u[k] = od * (1.f - tc * tc);
+    if (t < a.T && ch.live)
+      at(d0 + t * a.dgates_t + 2 * (int64_t)a.H, d_off) =
+          t < stop ? (E)(od * tc * (1.f - o)) : (E)0.f;
+  }
 #pragma unroll
-        for (int q = 0; q < W; ++q) {
-          const Pair p = back[0][q][lane];
-          sum = p.A * sum + p.C;
-          whole *= p.A;
-        }
-      carry = Chain(a).hand_on(order, ch, whole, sum, a.dcT, handed,
-                               begin == 0 ? a.dc0 : nullptr, w);
-    }
-    float now = carry = compose(carry, back[side], 0, rw);
+  for (int k = K - 1; k >= 0; --k) D = f[k] * (D + u[k]);
+  back[rw][lane] = {A, D};
+  __syncthreads();
+  float carry;
+  if (CHAIN) {
+    float whole = 1.f, sum = 0.f;
+    if (w == 0)
 #pragma unroll
-    for (int k = K - 1; k >= 0; --k) {
-      const int t = t0 + k;
-      const float dc = now + u[k], dci = dc * i[k], dcf = dc * f[k];
-      now = dcf;
-      if (t < end && ch.live) {
-        const bool on = t < stop;
-        E* d = d0 + t * a.dgates_t;
-        at(d, d_off) = on ? (E)(dci * n[k] * (1.f - i[k])) : (E)0.f;
-        at(d + a.H, d_off) =
-            on ? (E)(dcf * before[k] * (1.f - f[k])) : (E)0.f;
-        at(d + 3 * (int64_t)a.H, d_off) =
-            on ? (E)(dci * (1.f - n[k] * n[k])) : (E)0.f;
+      for (int q = 0; q < W; ++q) {
+        const Pair p = back[q][lane];
+        sum = p.A * sum + p.C;
+        whole *= p.A;
       }
+    carry = Chain(a).hand_on(slot.order, ch, whole, sum, a.dcT, handed,
+                             begin == 0 ? a.dc0 : nullptr, w);
+  } else {
+    carry = a.dcT ? a.dcT[ch.state] : 0.f;
+  }
+  carry = compose(carry, back, 0, rw);
+#pragma unroll
+  for (int k = K - 1; k >= 0; --k) {
+    const int t = t0 + k;
+    const float dc = carry + u[k], dci = dc * i[k], dcf = dc * f[k];
+    carry = dcf;
+    if (t < a.T && ch.live) {
+      const bool on = t < stop;
+      E* d = d0 + t * a.dgates_t;
+      at(d, d_off) = on ? (E)(dci * n[k] * (1.f - i[k])) : (E)0.f;
+      at(d + a.H, d_off) = on ? (E)(dcf * before[k] * (1.f - f[k])) : (E)0.f;
+      at(d + 3 * (int64_t)a.H, d_off) =
+          on ? (E)(dci * (1.f - n[k] * n[k])) : (E)0.f;
     }
-    if (!CHAIN) carry = compose(carry, back[side], rw, waves);
   }
   if (!CHAIN && w == 0 && ch.live) a.dc0[ch.state] = carry;
 }
@@ -467,15 +475,19 @@ void by_type(GlrType type, F f) {
   }
 }
 
-constexpr int STEPS = 8;        // of a wave in a tile
-constexpr int LOOP_WAVES = 8;
-// Up to 64 steps are one tile of waves with 4 steps each: more waves to hide
-// the one round of loads. 35 x 20 x 1500 bf16: 6.3 us against 6.8 with 8 steps
-// each, backward 8.6 against 9.4.
-constexpr int SHORT_STEPS = 4;
-constexpr int SHORT_WAVES = 16;  // at most
-constexpr int FWD_WAVES = 16;   // of a chain's blocks: the counter gives
-constexpr int BWD_WAVES = 8;    // a slot every 14 ns; 16 spill backward
+// Steps of a wave, and waves of a block. Up to 64 steps are a tile of waves
+// with 4 steps each (more waves to hide the one round of loads: 35 x 20 x 1500
+// bf16 takes 6.3 us against 6.8 with 8 each, 8.6 against 9.4 backward), up to
+// 128 one of waves with 8. A chain's tiles are 128 steps forward and 64
+// backward, with 16 a wave; half of that measured up to 20 % more where one
+// counter deals out the slots, at 14 ns a slot. Blocks that loop over tiles,
+// which need no chain, measured the same up to 128 steps, and from 256 steps
+// on up to four times a chain's time where channels are few (23 groups, 512
+// steps: 20 / 33 us against 10 / 14) and 1.1 to 1.4 times where they are many
+// (1875 groups, 512 steps: 161 / 401 against 153 / 292).
+constexpr int SHORT_STEPS = 4, MIDDLE_STEPS = 8, TILE_WAVES = 16;
+constexpr int CHAIN_STEPS = 16, FWD_WAVES = 8, BWD_WAVES = 4;
+constexpr int SHARED_FROM = 32;  // groups: a counter for each XCD
 
 // Rows of one launch: all, unless rows lie so far apart that those of a block
 // do not fit a lane's 32-bit offset; then one.
@@ -487,24 +499,13 @@ int rows_per_launch(const GlrArgs& a, int size) {
   return (apart * most + 4 * (int64_t)a.H) * size < (int64_t)1 << 32 ? a.B : 1;
 }
 
-// A loop over the tiles of 64 steps costs about 2.3 us a tile (4 backward)
-// as long as few blocks share the memory; a chain about 12 us, and then what
-// its bytes take at 3.3 to 3.8 TB/s, where a loop of many blocks reaches 4.4.
-// Measured, forward / backward in us, loop against chain: 24 groups of 64
-// channels, 4 tiles 12 / 19 against 12 / 13, 16 tiles 37 / 63 against 13 / 19;
-// 234 groups, 8 tiles 26 / 56 against 33 / 56; 375 groups, 16 tiles 80 / 171
-// against 73 / 146; 512 groups, 32 tiles 148 / 276 against 150 / 300.
-bool is_chain(const GlrArgs& a) {
-  const int tiles = cdiv(a.T, LOOP_WAVES * STEPS);
-  return a.groups < 448 && tiles > 4 + a.groups / 32;
-}
-
 GlrArgs planned(GlrArgs a, bool back, int size) {
   a.rows = rows_per_launch(a, size);
   a.groups = cdiv((int64_t)a.rows * a.H, 64);
-  a.chunks = is_chain(a)
-                 ? cdiv(a.T, (back ? BWD_WAVES : FWD_WAVES) * STEPS)
+  a.chunks = a.T > MIDDLE_STEPS * TILE_WAVES
+                 ? cdiv(a.T, (back ? BWD_WAVES : FWD_WAVES) * CHAIN_STEPS)
                  : 0;
+  a.counters_log2 = a.groups < SHARED_FROM ? 0 : COUNTERS_LOG2;
   return a;
 }
 
@@ -517,20 +518,22 @@ void launch(const GlrArgs& args, hipStream_t stream) {
       const int64_t n = glr_work_words(args, BACK, sizeof(E)) / 2;
       hipLaunchKernelGGL(glr_reset_kernel, dim3(cdiv(n, 256)), dim3(256), 0,
                          stream, reinterpret_cast<uint4*>(a.work), n);
-      auto kernel = BACK ? glr_bwd_kernel<E, STEPS, CHAIN_W, true>
-                         : glr_fwd_kernel<E, STEPS, CHAIN_W, true>;
-      hipLaunchKernelGGL(kernel, dim3(a.groups * a.chunks),
+      auto kernel = BACK ? glr_bwd_kernel<E, CHAIN_STEPS, CHAIN_W, true>
+                         : glr_fwd_kernel<E, CHAIN_STEPS, CHAIN_W, true>;
+      const int counters = 1 << a.counters_log2;
+      const int blocks = counters * cdiv(a.groups, counters) * a.chunks;
+      hipLaunchKernelGGL(kernel, dim3(blocks),
                          dim3(64 * CHAIN_W), 0, stream, a);
-    } else if (a.T <= SHORT_STEPS * SHORT_WAVES) {
-      auto kernel = BACK ? glr_bwd_kernel<E, SHORT_STEPS, SHORT_WAVES, false>
-                         : glr_fwd_kernel<E, SHORT_STEPS, SHORT_WAVES, false>;
+    } else if (a.T <= SHORT_STEPS * TILE_WAVES) {
+      auto kernel = BACK ? glr_bwd_kernel<E, SHORT_STEPS, TILE_WAVES, false>
+                         : glr_fwd_kernel<E, SHORT_STEPS, TILE_WAVES, false>;
       hipLaunchKernelGGL(kernel, dim3(a.groups),
                          dim3(64 * cdiv(a.T, SHORT_STEPS)), 0, stream, a);
     } else {
-      auto kernel = BACK ? glr_bwd_kernel<E, STEPS, LOOP_WAVES, false>
-                         : glr_fwd_kernel<E, STEPS, LOOP_WAVES, false>;
-      hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(64 * LOOP_WAVES), 0,
-                         stream, a);
+      auto kernel = BACK ? glr_bwd_kernel<E, MIDDLE_STEPS, TILE_WAVES, false>
+                         : glr_fwd_kernel<E, MIDDLE_STEPS, TILE_WAVES, false>;
+      hipLaunchKernelGGL(kernel, dim3(a.groups),
+                         dim3(64 * cdiv(a.T, MIDDLE_STEPS)), 0, stream, a);
     }
   }
 }

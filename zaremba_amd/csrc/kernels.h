@@ -78,7 +78,6 @@ void launch_lstm_persistent_bwd(const bf16* dY, const bf16* rec,
 // the state of launch_glr_step (cT, read and written), whose rows are c_b
 // apart.
 constexpr int GLR_MARK = 32;  // steps between two kept states
-constexpr int GLR_COUNTER_WORDS = 32;
 enum class GlrType { F32, F16, BF16 };
 struct GlrArgs {
   const void* gates = nullptr;  // [T, B, 4H]
@@ -102,6 +101,7 @@ struct GlrArgs {
   // set by the launchers: the rows of a launch, its blocks of 64 channels
   // and chunks of time
   int row0 = 0, rows = 0, groups = 0, chunks = 0;
+  int counters_log2 = 0;
 };
 // Words of 64 bits that a call needs for itself; size: of a gate in bytes.
 int64_t glr_work_words(const GlrArgs& a, bool back, int size);
