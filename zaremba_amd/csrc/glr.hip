@@ -171,8 +171,8 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 // but 23.4 x 65536 265 / 552 against 274 / 575, where an XCD has 3 groups.
 //
 // At T = 65536, B = 1, H = 1500, bf16 this takes 259 us forward (983 MB, 3.8
-// TB/s of the 5.2 that a copy reaches) and 566 backward (1770 MB, 3.1 TB/s);
-// with rows of whole lines, H = 1472, 203 (4.8 TB/s) and 373 (4.7). Vector
+// TB/s of the 5.2 that a copy reaches) and 545 backward (1770 MB, 3.2 TB/s);
+// with rows of whole lines, H = 1472, 201 (4.8 TB/s) and 368 (4.7). Vector
 // instructions take half of either. Before, finding the (A, C) of long chunks
 // in a launch of its own, which reads three gates twice, took 360 and 680, and
 // a block that loops over its tiles 2380 and 4500.
@@ -478,15 +478,17 @@ void by_type(GlrType type, F f) {
 // Steps of a wave, and waves of a block. Up to 64 steps are a tile of waves
 // with 4 steps each (more waves to hide the one round of loads: 35 x 20 x 1500
 // bf16 takes 6.3 us against 6.8 with 8 each, 8.6 against 9.4 backward), up to
-// 128 one of waves with 8. A chain's tiles are 128 steps forward and 64
-// backward, with 16 a wave; half of that measured up to 20 % more where one
-// counter deals out the slots, at 14 ns a slot. Blocks that loop over tiles,
+// 128 one of waves with 8. A chain's tiles are 128 steps forward, 64 backward,
+// of 8 waves. 16 waves with 8 steps measured 218 us against 200 forward at
+// 65536 x 1 x 1472, 4 waves with 16 566 against 545 backward at 65536 x 1 x
+// 1500; half the tile up to 20 % more where one counter deals out the slots,
+// at 14 ns a slot. Blocks that loop over tiles,
 // which need no chain, measured the same up to 128 steps, and from 256 steps
 // on up to four times a chain's time where channels are few (23 groups, 512
 // steps: 20 / 33 us against 10 / 14) and 1.1 to 1.4 times where they are many
 // (1875 groups, 512 steps: 161 / 401 against 153 / 292).
 constexpr int SHORT_STEPS = 4, MIDDLE_STEPS = 8, TILE_WAVES = 16;
-constexpr int CHAIN_STEPS = 16, FWD_WAVES = 8, BWD_WAVES = 4;
+constexpr int FWD_STEPS = 16, BWD_STEPS = 8, CHAIN_WAVES = 8;
 constexpr int SHARED_FROM = 32;  // groups: a counter for each XCD
 
 // Rows of one launch: all, unless rows lie so far apart that those of a block
@@ -503,7 +505,7 @@ GlrArgs planned(GlrArgs a, bool back, int size) {
   a.rows = rows_per_launch(a, size);
   a.groups = cdiv((int64_t)a.rows * a.H, 64);
   a.chunks = a.T > MIDDLE_STEPS * TILE_WAVES
-                 ? cdiv(a.T, (back ? BWD_WAVES : FWD_WAVES) * CHAIN_STEPS)
+                 ? cdiv(a.T, (back ? BWD_STEPS : FWD_STEPS) * CHAIN_WAVES)
                  : 0;
   a.counters_log2 = a.groups < SHARED_FROM ? 0 : COUNTERS_LOG2;
   return a;
@@ -511,19 +513,18 @@ GlrArgs planned(GlrArgs a, bool back, int size) {
 
 template <bool BACK, typename E>
 void launch(const GlrArgs& args, hipStream_t stream) {
-  constexpr int CHAIN_W = BACK ? BWD_WAVES : FWD_WAVES;
   GlrArgs a = planned(args, BACK, sizeof(E));
   for (a.row0 = 0; a.row0 < a.B; a.row0 += a.rows) {
     if (a.chunks) {
       const int64_t n = glr_work_words(args, BACK, sizeof(E)) / 2;
       hipLaunchKernelGGL(glr_reset_kernel, dim3(cdiv(n, 256)), dim3(256), 0,
                          stream, reinterpret_cast<uint4*>(a.work), n);
-      auto kernel = BACK ? glr_bwd_kernel<E, CHAIN_STEPS, CHAIN_W, true>
-                         : glr_fwd_kernel<E, CHAIN_STEPS, CHAIN_W, true>;
+      auto kernel = BACK ? glr_bwd_kernel<E, BWD_STEPS, CHAIN_WAVES, true>
+                         : glr_fwd_kernel<E, FWD_STEPS, CHAIN_WAVES, true>;
       const int counters = 1 << a.counters_log2;
       const int blocks = counters * cdiv(a.groups, counters) * a.chunks;
       hipLaunchKernelGGL(kernel, dim3(blocks),
-                         dim3(64 * CHAIN_W), 0, stream, a);
+                         dim3(64 * CHAIN_WAVES), 0, stream, a);
     } else if (a.T <= SHORT_STEPS * TILE_WAVES) {
       auto kernel = BACK ? glr_bwd_kernel<E, SHORT_STEPS, TILE_WAVES, false>
                          : glr_fwd_kernel<E, SHORT_STEPS, TILE_WAVES, false>;
