@@ -220,12 +220,14 @@ def refusals(device):
             x["step"], lr=x.get("lr", 0.1), betas=x.get("betas", (0.9, 0.99)),
             eps=x.get("eps", 1e-8), weight_decay=x.get("wd", 0.0),
             max_norm=x.get("max_norm"), shadows=x["shadows"],
+            grad_scale=x.get("grad_scale", 1.0),
             exp_avg_scales=x.get("exp_avg_scales"))
 
     nothing = lambda x: None  # noqa: E731
     return [call(nothing, lr=-1.0), call(nothing, betas=(0.9, 1.0)),
             call(nothing, eps=0.0), call(nothing, wd=-1.0),
             call(nothing, max_norm=0.0), call(nothing, lr=float("nan")),
+            call(nothing, grad_scale=0.0), call(nothing, grad_scale=-1.0),
             call(nothing, exp_avg_scales=[torch.zeros(1, device=device)] * 2),
             call(nothing, params=[]), call(lambda x: x["grads"].pop()),
             call(lambda x: x["shadows"].pop())]
@@ -502,3 +504,49 @@ def test_another_stream():
         check(y)
     st.synchronize()
     assert torch.equal(x["params"][0], y["params"][0])
+
+
+@GPU
+def test_writes_are_seen_by_autograd():
+    x = make([30], "cuda")
+    p = x["params"][0].requires_grad_()
+    y = (p * p).sum()
+    A.adamw_step_(x["params"], x["grads"], x["exp_avgs"], x["exp_avg_sqs"],
+                  x["step"], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+
+
+@GPU
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_of_over_two_to_the_31(bits):
+    """Offsets past 32 bits: the last values of a tensor of 2^31 + 300 follow
+    those of a short one that holds the same."""
+    n, k = (1 << 31) + 300, 300 + 256
+    gen = torch.Generator().manual_seed(1)
+    tail = {name: torch.randn(k, generator=gen).cuda()
+            for name in ("p", "g", "m")}
+    big = {name: torch.zeros(n, device="cuda") for name in ("p", "g")}
+    for name in ("p", "g"):
+        big[name][-k:] = tail[name]
+    kind = torch.float32 if bits == 32 else E4M3
+    state = lambda n: torch.zeros(  # noqa: E731
+        n, dtype=torch.float32 if bits == 32 else torch.uint8,
+        device="cuda").view(kind)
+    scales = lambda n: None if bits == 32 else [  # noqa: E731
+        torch.zeros(-(-n // 256), device="cuda")]
+
+    def run(p, g, n):
+        m, v, ms, vs = state(n), state(n), scales(n), scales(n)
+        st = torch.zeros(1, dtype=torch.int64, device="cuda")
+        norm = A.adamw_step_([p], [g], [m], [v], st, lr=0.1, max_norm=1.0,
+                             exp_avg_scales=ms, exp_avg_sq_scales=vs)
+        return p[-k:], m[-k:].float(), norm
+
+    a = run(big["p"], big["g"], n)
+    # the short tensor ends as the long one does: 300 into a block of 256
+    pad = torch.zeros(44 + 212, device="cuda")
+    b = run(torch.cat([pad, tail["p"]]), torch.cat([pad, tail["g"]]), 256 + k)
+    for u, v in zip(a, b):
+        assert torch.equal(u, v)
+    assert not bool(big["p"][:-k].any())

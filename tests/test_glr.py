@@ -214,6 +214,12 @@ def test_refusals_gpu():
             lambda: G.glr_forward(gates, c0.cpu()),
             lambda: G.glr_forward(gates, c0, torch.tensor([1, 2, 3])),
             lambda: G.glr_forward(gates, c0, out=gates[..., :2]),
+            lambda: G.glr_forward(gates, c0, out=gates.view(-1)[:24].view(
+                4, 3, 2)),
+            lambda: G.glr_backward(dh, dcT, gates, c0, marks, out=gates),
+            lambda: G.glr_backward(dh, dcT, gates, c0, marks,
+                                   out=gates[:3].clone()),
+            lambda: G.glr_step(gates[0], gates.view(-1)[:6].view(3, 2)),
             lambda: G.glr_backward(dh.half(), dcT, gates, c0, marks),
             lambda: G.glr_backward(dh[:2], dcT, gates, c0, marks),
             lambda: G.glr_backward(dh, dcT, gates, c0, marks[..., :1]),
@@ -311,13 +317,35 @@ def test_closed_and_open_gates(dtype):
 
 
 @GPU
-def test_nan_stays_in_its_channel():
-    gates, c0, *_ = make(70, 3, 9, torch.float32, "cuda")
+@pytest.mark.parametrize("T", [70, 700])
+def test_nan_stays_in_its_channel(T):
+    """In one tile, and through a chain, forward and backward."""
+    gates, c0, dh, dcT, _ = make(T, 3, 9, torch.float32, "cuda")
     gates[30, 1, 4] = float("nan")
-    h, cT, _ = G.glr_forward(gates, c0)
+    h, cT, marks = G.glr_forward(gates, c0, training=True)
     bad = torch.isnan(h)
-    assert bool(bad[30:, 1, 4].all()) and int(bad.sum()) == 40
+    assert bool(bad[30:, 1, 4].all()) and int(bad.sum()) == T - 30
     assert int(torch.isnan(cT).sum()) == 1
+    dh[20, 0, 7] = float("nan")
+    d, dc0 = G.glr_backward(dh, dcT, gates, c0, marks)
+    bad = torch.isnan(d.view(T, 3, 4, 9)).any(2)
+    assert bool(bad[:, 1, 4].all())          # NaN states give NaN gradients
+    assert bool(bad[:21, 0, 7].all()) and int(bad[:, 0, 7].sum()) == 21
+    assert int(bad.sum()) == T + 21
+    assert int(torch.isnan(dc0).sum()) == 2
+
+
+@GPU
+def test_writes_are_seen_by_autograd():
+    """A tensor that a graph has saved and a kernel then overwrites."""
+    gates, c0, *_ = make(4, 3, 2, torch.float32, "cuda")
+    w = torch.ones(3, 2, device="cuda", requires_grad=True)
+    c = c0.clone()
+    y = (w * c).sum()
+    with torch.no_grad():
+        G.glr_step(gates[0], c)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
 
 
 @GPU

@@ -253,7 +253,7 @@ def test_hip_adamw_trains(cell, bits):
         for p, q in zip(m.parameters(), twin):
             # lr times 30 half steps a step (tests/test_adamw.py); in 8 bits
             # a draw next to its border may move a code, 1 / 8 of a value
-            off = (p.detach().cpu() - q).abs()
+            off = (p.detach().cpu() - q.detach()).abs()
             if bits == 32:
                 assert float(off.max()) < (step + 1) * 32 * 2.0 ** -24
             else:

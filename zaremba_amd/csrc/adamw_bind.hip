@@ -73,7 +73,10 @@ OptTensor adamw_step_(const Tensors& params, const Tensors& grads,
   // what is written, as ranges of addresses
   std::vector<std::pair<const char*, const char*>> written;
   written.reserve(6 * count);
+  std::vector<const Tensor*> to_bump;
+  to_bump.reserve(6 * count + 1);
   auto writes = [&](const Tensor& x) {
+    to_bump.push_back(&x);
     const char* at = static_cast<const char*>(x.data_ptr());
     if (x.numel()) written.emplace_back(at, at + x.nbytes());
   };
@@ -185,6 +188,7 @@ OptTensor adamw_step_(const Tensors& params, const Tensors& grads,
                        : torch::empty({}, first.options());
     w.norm = norm.data_ptr<float>();
   }
+  for (const Tensor* x : to_bump) x->unsafeGetTensorImpl()->bump_version();
   const auto stream = current_stream();
   int done = 0;
   for (const auto& a : launches) {

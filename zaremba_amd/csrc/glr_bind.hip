@@ -7,6 +7,7 @@
 
 #include <limits>
 #include <tuple>
+#include <utility>
 
 #include "bind.h"
 #include "kernels.h"
@@ -72,6 +73,31 @@ void set_lengths(GlrArgs& a, const OptTensor& lengths, Tensor& keep,
   a.lengths_64 = keep.scalar_type() == torch::kInt64;
 }
 
+// Whether two tensors' ranges of addresses meet.
+bool overlap(const Tensor& a, const Tensor& b) {
+  auto range = [](const Tensor& t) {
+    const char* at = static_cast<const char*>(t.data_ptr());
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d)
+      last += (t.size(d) - 1) * t.stride(d);
+    return std::make_pair(at, at + (last + 1) * t.element_size());
+  };
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto x = range(a), y = range(b);
+  return x.first < y.second && y.first < x.second;
+}
+
+void check_out(const Tensor& out, const Tensor& gates, int64_t width,
+               const char* op) {
+  TORCH_CHECK(out.scalar_type() == gates.scalar_type() &&
+              out.device() == gates.device() && out.dim() == 3 &&
+              out.size(0) == gates.size(0) && out.size(1) == gates.size(1) &&
+              out.size(2) == width && out.is_contiguous(),
+              op, ": out must be a contiguous [", gates.size(0), ", ",
+              gates.size(1), ", ", width, "] of the gates' type and device");
+  TORCH_CHECK(!overlap(out, gates), op, ": out shares memory with gates");
+}
+
 Tensor dense_rows(const Tensor& t) {
   return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous();
 }
@@ -124,12 +150,8 @@ std::tuple<Tensor, Tensor, OptTensor> glr_forward(
   Tensor h;
   if (out) {
     h = *out;
-    TORCH_CHECK(h.scalar_type() == gates.scalar_type() &&
-                h.device() == gates.device() && h.dim() == 3 &&
-                h.size(0) == a.T && h.size(1) == a.B && h.size(2) == a.H &&
-                h.is_contiguous(),
-                op, ": out must be a contiguous [T, B, H] of the gates' type "
-                "and device");
+    check_out(h, gates, a.H, op);
+    h.unsafeGetTensorImpl()->bump_version();
   } else {
     h = empty_as(gates, a.H);
   }
@@ -197,11 +219,9 @@ std::tuple<Tensor, Tensor> glr_backward(
   Tensor dgates;
   if (out) {
     dgates = *out;
-    TORCH_CHECK(dgates.scalar_type() == gates.scalar_type() &&
-                dgates.device() == gates.device() &&
-                dgates.sizes() == gates.sizes() && dgates.is_contiguous(),
-                op, ": out must be a contiguous tensor of the gates' size, "
-                "type and device");
+    check_out(dgates, gates, 4 * (int64_t)a.H, op);
+    TORCH_CHECK(!overlap(dgates, dh), op, ": out shares memory with dh");
+    dgates.unsafeGetTensorImpl()->bump_version();
   } else {
     dgates = empty_as(gates, 4 * (int64_t)a.H);
   }
@@ -250,8 +270,10 @@ Tensor glr_step(const Tensor& gates_in, const Tensor& c) {
               (a.B <= 1 || c.stride(0) >= a.H),
               op, ": the rows of c must be dense and apart, got strides ",
               c.strides());
+  TORCH_CHECK(!overlap(c, gates), op, ": c shares memory with gates");
   Tensor h = torch::empty({a.B, a.H}, gates.options());
   if (h.numel() == 0) return h;
+  c.unsafeGetTensorImpl()->bump_version();
   a.gates = gates.data_ptr();
   a.gates_b = gates.stride(0);
   a.h = h.data_ptr();

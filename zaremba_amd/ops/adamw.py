@@ -34,7 +34,7 @@ E4M3 = torch.float8_e4m3fn
 BLOCK = 256
 
 
-def _check(lr, betas, eps, weight_decay, max_norm):
+def _check(lr, betas, eps, weight_decay, max_norm, grad_scale=1.0):
     if not lr >= 0:
         raise ValueError(f"adamw_step_: lr must not be negative, got {lr}")
     if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
@@ -47,6 +47,9 @@ def _check(lr, betas, eps, weight_decay, max_norm):
     if max_norm is not None and not max_norm > 0:
         raise ValueError("adamw_step_: max_norm must be positive or None, "
                          f"got {max_norm}")
+    if not grad_scale > 0:
+        raise ValueError("adamw_step_: grad_scale must be positive, got "
+                         f"{grad_scale}")
 
 
 @torch.no_grad()
@@ -65,7 +68,7 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr,
     Returns the gradient norm before the clip (0-d float32), None where
     ``max_norm`` is None: nothing is clipped then, and no norm computed.
     """
-    _check(lr, betas, eps, weight_decay, max_norm)
+    _check(lr, betas, eps, weight_decay, max_norm, grad_scale)
     if len(params) == 0:
         raise RuntimeError("adamw_step_: no parameters")
     if params[0].is_cuda and not _C.force_eager_env():
@@ -90,7 +93,9 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr,
 
 class AdamW:
     """The states of a model's parameters, in the order of
-    ``model.parameters()``. ``trainer.adamw_step`` makes the step."""
+    ``model.parameters()``. ``trainer.adamw_step`` makes the step; on the HIP
+    engine it is what rewrites the bf16 shadows, too, that the next forward
+    reads, so ``step`` alone is for parameters without shadows."""
 
     def __init__(self, params, betas=(0.9, 0.999), eps=1e-8,
                  weight_decay=0.01, bits=32):

@@ -12,8 +12,8 @@ Types and layouts
     last axis is dense; time and batch may have any strides (batch-first
     storage is ``x.transpose(0, 1)``). ``h`` and ``dgates`` are stored in the
     order of ``gates``.
-  * states (``c0``, ``cT`` and their gradients): float32 [B, H]. ``None``
-    stands for zeros.
+  * states (``c0``, ``cT`` and their gradients): float32 [B, H], finite.
+    ``None`` stands for zeros. A NaN stays in its channel, from its step on.
   * ``lengths``: int32 or int64 [B] on the same device, values outside
     [0, T] count as the nearer end. From ``lengths[b]`` on row b keeps its
     state, its ``h`` and ``dgates`` are zero, and what stands in ``gates``
@@ -21,7 +21,10 @@ Types and layouts
 
 On the GPU every function runs the HIP kernels on the current stream of the
 tensors' device; on the CPU (or with ZAREMBA_AMD_FORCE_EAGER=1) it runs the
-eager math of ops/functional.py. All of them may be captured in a HIP graph.
+eager math of ops/functional.py. All of them may be captured in a HIP graph;
+a captured training step calls glr_forward and glr_backward themselves, which
+need no autograd. Windows of up to 128 steps are one launch; longer ones two,
+with a workspace of 8 bytes for each channel and 128 steps (64 backward).
 """
 
 from __future__ import annotations
