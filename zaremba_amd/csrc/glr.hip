@@ -23,7 +23,7 @@
 //
 // A lane has one channel, so that rows may have any length and alignment. Two
 // channels a lane, with loads twice as wide, measured 264 to 290 us against
-// 260 forward and 521 to 576 against 533 backward at 65536 x 1 x 1500 bf16:
+// 260 forward and 521 to 576 against 545 backward at 65536 x 1 x 1500 bf16:
 // the registers of twice the steps leave half the waves.
 #include <algorithm>
 #include <cmath>
@@ -158,7 +158,7 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 // no order between stores is needed, and words go past the L2s, which do not
 // see each other's writes.
 //
-// Blocks take their slots from a counter as they start. A block therefore
+// Blocks take their slots from counters as they start. A block therefore
 // waits only for blocks that run already, and these only for earlier ones:
 // every wait ends, whatever the number of blocks that fit the chip. Polls are
 // bounded all the same; behind a bound that is reached the state is NaN.
@@ -166,21 +166,27 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 // From SHARED_FROM groups of 64 channels on each of the 8 XCDs has a counter
 // and a share of the groups, neighbours side by side: rows of 64 values are
 // seldom whole cache lines, and the other halves are then met in the same L2.
-// Measured in us, forward / backward, one counter against eight: 375 groups x
-// 1024 steps 77 / 153 against 64 / 120, 94 x 4096 76 / 148 against 66 / 126;
-// but 23.4 x 65536 265 / 552 against 274 / 575, where an XCD has 3 groups.
+// With fewer groups each has a counter of its own, as the blocks of one would
+// queue at one address (14 ns a slot) and an XCD would have 3 groups or less.
+// Measured in us, forward / backward, bf16, H = 1500: with a counter a group
+// against shares, 23.4 groups x 65536 steps 250 / 537 against 276 / 578 (one
+// counter for all: 260 / 545), 15.6 x 16384 (H = 1000) 53 / 90 against 52 / 99,
+// but 94 x 4096 69 / 141 against 65 / 120 and 375 x 1024 70 / 146 against 62 /
+// 113.
 //
-// At T = 65536, B = 1, H = 1500, bf16 this takes 259 us forward (983 MB, 3.8
-// TB/s of the 5.2 that a copy reaches) and 545 backward (1770 MB, 3.2 TB/s);
-// with rows of whole lines, H = 1472, 201 (4.8 TB/s) and 368 (4.7). Vector
+// At T = 65536, B = 1, H = 1500, bf16 this takes 250 us forward (983 MB, 3.9
+// TB/s of the 5.2 that a copy reaches) and 537 backward (1770 MB, 3.3 TB/s);
+// with rows of whole lines, H = 1472, 201 (4.8 TB/s) and 353 (4.9). The rest is
+// lines that two XCDs read: 1.6 and 1.8 times the bytes at H = 1500. Vector
 // instructions take half of either. Before, finding the (A, C) of long chunks
 // in a launch of its own, which reads three gates twice, took 360 and 680, and
 // a block that loops over its tiles 2380 and 4500.
 constexpr unsigned ABSENT = 0xffffffffu;
 constexpr int MOST_POLLS = 1 << 22;
-constexpr int COUNTERS_LOG2 = 3;   // one counter, or one for each XCD
+constexpr int XCDS = 8;
+constexpr int SHARED_FROM = 32;    // groups: a counter for each XCD
 constexpr int COUNTER_APART = 16;  // words: 128 bytes
-constexpr int COUNTER_WORDS = COUNTER_APART << COUNTERS_LOG2;  // go first
+constexpr int COUNTER_WORDS = COUNTER_APART * SHARED_FROM;  // go first
 constexpr int DEPTH = 4;
 
 DEV_INLINE unsigned to_bits(float x) {  // any NaN but ABSENT
@@ -199,22 +205,20 @@ struct Chain {
   DEV_INLINE Chain(const GlrArgs& a)
       : words(a.work + COUNTER_WORDS), BH((int64_t)a.B * a.H) {}
 
-  // Counter x deals out the slots of its own share of the groups.
+  // A counter deals out the slots of its groups in order. It gets at least as
+  // many blocks as slots: order a.chunks is none.
   static DEV_INLINE Slot take_slot(const GlrArgs& a, int* lds) {
-    const int x = blockIdx.x & ((1 << a.counters_log2) - 1);
+    const bool shared = a.groups >= SHARED_FROM;
+    const int x = shared ? blockIdx.x % XCDS : blockIdx.x / XCDS % a.groups;
     if (threadIdx.x == 0)
       *lds = (int)__hip_atomic_fetch_add(
           reinterpret_cast<unsigned*>(a.work + x * COUNTER_APART), 1u,
           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int first = a.groups * x >> a.counters_log2;
-    const int n = (a.groups * (x + 1) >> a.counters_log2) - first;
+    const int first = shared ? a.groups * x / XCDS : x;
+    const int n = shared ? a.groups * (x + 1) / XCDS - first : 1;
     __syncthreads();
     const int k = __builtin_amdgcn_readfirstlane(*lds);
-    // a share may be smaller than the largest: order a.chunks is none
-    Slot s;
-    s.order = n ? min(k / n, a.chunks) : a.chunks;
-    s.group = first + (n ? k % n : 0);
-    return s;
+    return {min(k / n, a.chunks), first + k % n};
   }
 
   DEV_INLINE void publish(int slot, const Channel& ch, float A,
@@ -481,15 +485,12 @@ void by_type(GlrType type, F f) {
 // 128 one of waves with 8. A chain's tiles are 128 steps forward, 64 backward,
 // of 8 waves. 16 waves with 8 steps measured 218 us against 200 forward at
 // 65536 x 1 x 1472, 4 waves with 16 566 against 545 backward at 65536 x 1 x
-// 1500; half the tile up to 20 % more where one counter deals out the slots,
-// at 14 ns a slot. Blocks that loop over tiles,
-// which need no chain, measured the same up to 128 steps, and from 256 steps
+// 1500. Blocks that loop over tiles, which need no chain, measured the same up to 128 steps, and from 256 steps
 // on up to four times a chain's time where channels are few (23 groups, 512
 // steps: 20 / 33 us against 10 / 14) and 1.1 to 1.4 times where they are many
 // (1875 groups, 512 steps: 161 / 401 against 153 / 292).
 constexpr int SHORT_STEPS = 4, MIDDLE_STEPS = 8, TILE_WAVES = 16;
 constexpr int FWD_STEPS = 16, BWD_STEPS = 8, CHAIN_WAVES = 8;
-constexpr int SHARED_FROM = 32;  // groups: a counter for each XCD
 
 // Rows of one launch: all, unless rows lie so far apart that those of a block
 // do not fit a lane's 32-bit offset; then one.
@@ -507,7 +508,6 @@ GlrArgs planned(GlrArgs a, bool back, int size) {
   a.chunks = a.T > MIDDLE_STEPS * TILE_WAVES
                  ? cdiv(a.T, (back ? BWD_STEPS : FWD_STEPS) * CHAIN_WAVES)
                  : 0;
-  a.counters_log2 = a.groups < SHARED_FROM ? 0 : COUNTERS_LOG2;
   return a;
 }
 
@@ -521,8 +521,9 @@ void launch(const GlrArgs& args, hipStream_t stream) {
                          stream, reinterpret_cast<uint4*>(a.work), n);
       auto kernel = BACK ? glr_bwd_kernel<E, BWD_STEPS, CHAIN_WAVES, true>
                          : glr_fwd_kernel<E, FWD_STEPS, CHAIN_WAVES, true>;
-      const int counters = 1 << a.counters_log2;
-      const int blocks = counters * cdiv(a.groups, counters) * a.chunks;
+      const int blocks =
+          a.groups >= SHARED_FROM ? XCDS * cdiv(a.groups, XCDS) * a.chunks
+                                  : XCDS * cdiv(a.chunks, XCDS) * a.groups;
       hipLaunchKernelGGL(kernel, dim3(blocks),
                          dim3(64 * CHAIN_WAVES), 0, stream, a);
     } else if (a.T <= SHORT_STEPS * TILE_WAVES) {

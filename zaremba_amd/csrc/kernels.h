@@ -101,7 +101,6 @@ struct GlrArgs {
   // set by the launchers: the rows of a launch, its blocks of 64 channels
   // and chunks of time
   int row0 = 0, rows = 0, groups = 0, chunks = 0;
-  int counters_log2 = 0;
 };
 // Words of 64 bits that a call needs for itself; size: of a gate in bytes.
 int64_t glr_work_words(const GlrArgs& a, bool back, int size);
