@@ -528,3 +528,40 @@ def test_rows_further_apart_than_an_offset_reaches(T):
     d2, dc02 = G.glr_backward(dh, dcT, src, c0, marks2, lengths)
     for a, b in ((h, h2), (cT, cT2), (d, d2), (dc0, dc02)):
         near(a, b.double().cpu(), 16.0, "far rows")
+
+
+@GPU
+@pytest.mark.parametrize("T,B,H", [(40000, 1, 96), (3000, 9, 300)])
+def test_same_bits_whatever_else_runs(T, B, H):
+    """A long window is many blocks that wait for each other in an order that
+    other work changes; its roundings are the same."""
+    gates, c0, dh, dcT, _ = make(T, B, H, torch.float32, "cuda")
+    load = torch.randn(1 << 24, device="cuda")
+    side = torch.cuda.Stream()
+    first = None
+    for _ in range(12):
+        with torch.cuda.stream(side):
+            for _ in range(6):
+                load.mul_(0.999)
+        h, cT, marks = G.glr_forward(gates, c0, training=True)
+        got = (h, cT, marks) + G.glr_backward(dh, dcT, gates, c0, marks)
+        first = first or got
+        assert all(torch.equal(x, y) for x, y in zip(got, first))
+    torch.cuda.synchronize()
+
+
+@GPU
+@pytest.mark.parametrize("H", [9, 64, 70])
+@pytest.mark.parametrize("ends", [
+    [0, 1, 63, 64, 65, 127, 128, 129, 255, 256, 257, 383, 384, 385, 399, 400],
+    [0] * 15 + [1], [128] * 16, [1, 400] * 8, [0] * 16])
+def test_rows_that_end_at_tiles(H, ends):
+    """Whole tiles of padding, with NaN there, and no step of some rows."""
+    T, B = 400, len(ends)
+    gates, c0, dh, dcT, _ = make(T, B, H, torch.bfloat16, "cuda")
+    lengths = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    live = (torch.arange(T, device="cuda")[:, None]
+            < lengths[None])[..., None]
+    gates = gates.masked_fill(~live, float("nan"))
+    dh = dh.masked_fill(~live, float("nan"))
+    check(gates, c0, dh, dcT, lengths)

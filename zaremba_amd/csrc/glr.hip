@@ -76,24 +76,28 @@ struct Channel {
   int first;      // row of the block's first lane
   int row;        // this lane's row, less `first`
   int j;
-  bool live;      // a lane behind the last channel repeats the block's first
   int n_live;     // steps of the row
+  int most;       // steps of the block's longest row
   int64_t state;  // place in a [B, H]
 
   DEV_INLINE Channel(const GlrArgs& a, int group) {
     const int id0 = group * 64, id = id0 + lane_id();
-    live = id < a.rows * a.H;
-    const int b0 = id0 / a.H, r = (live ? id : id0) - b0 * a.H;
+    // a lane behind the last channel repeats the block's first, with its stores
+    const int b0 = id0 / a.H, r = (id < a.rows * a.H ? id : id0) - b0 * a.H;
     first = a.row0 + b0;
     row = a.H >= 64 ? r >= a.H : r / a.H;
     j = r - row * a.H;
     state = (int64_t)(first + row) * a.H + j;
-    n_live = a.T;
+    n_live = most = a.T;
     if (a.lengths) {
       const int64_t n = a.lengths_64
                             ? static_cast<const int64_t*>(a.lengths)[first + row]
                             : static_cast<const int*>(a.lengths)[first + row];
       n_live = (int)(n < 0 ? 0 : n > a.T ? a.T : n);
+      int m = n_live;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) m = max(m, __shfl_xor(m, d));
+      most = __builtin_amdgcn_readfirstlane(m);
     }
   }
 
@@ -108,16 +112,17 @@ template <typename E, int K>
 struct Gates {
   E i[K], f[K], o[K], n[K];
 
-  // Steps [t0, t0 + K); those past T read the last one.
+  // Steps [t0, t0 + K); those past `last` read it instead.
   DEV_INLINE void load(const GlrArgs& a, const E* base, unsigned offset,
-                       int t0) {
+                       int t0, int last) {
+    const E* p = base + (int64_t)min(t0, last) * a.gates_t;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const E* p = base + (int64_t)min(t0 + k, a.T - 1) * a.gates_t;
       i[k] = at(p, offset);
       f[k] = at(p + a.H, offset);
       o[k] = at(p + 2 * (int64_t)a.H, offset);
       n[k] = at(p + 3 * (int64_t)a.H, offset);
+      p += t0 + k < last ? a.gates_t : 0;
     }
   }
 
@@ -153,10 +158,22 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 // scan, has a word for each channel. It first publishes its (A, C) there and,
 // once it knows the state before it, the state behind it instead, marked by
 // A = -1. A wave looks back over the slots before its own, DEPTH of them at a
-// time, and composes their pairs until it meets a state. A word says by itself
-// whether it is there (all ones: not yet; no word that is written is), so that
-// no order between stores is needed, and words go past the L2s, which do not
-// see each other's writes.
+// time, keeps up to SEEN pairs until it meets a state, and then composes them
+// from that state on: the same roundings in the same order whichever state it
+// was, so that results do not depend on when a block runs. A word says by
+// itself whether it is there (all ones: not yet; no word that is written is),
+// so that no order between stores is needed, and words go past the L2s, which
+// do not see each other's writes. Looking at 1 or 4 words at a time, or
+// keeping 16, measured the same within 2 %; keeping 4 takes 5 % longer at
+// 16384 x 1 x 1000.
+//
+// A tile behind the last step of each of its rows writes zeros and ends; the
+// chain ends, or in the backward pass begins, with the tile before. Rows of
+// random lengths, forward / backward: 133 / 243 us against 155 / 279 with such
+// tiles in the chain at 512 x 80 x 1500, 28 / 55 against 35 / 59 at 1001 x 17 x
+// 651. Their reads are half of all; an XCD whose rows are short then waits for
+// the others, and dealing groups out in smaller pieces costs as much in lines
+// that two XCDs read.
 //
 // Blocks take their slots from counters as they start. A block therefore
 // waits only for blocks that run already, and these only for earlier ones:
@@ -187,7 +204,7 @@ constexpr int XCDS = 8;
 constexpr int SHARED_FROM = 32;    // groups: a counter for each XCD
 constexpr int COUNTER_APART = 16;  // words: 128 bytes
 constexpr int COUNTER_WORDS = COUNTER_APART * SHARED_FROM;  // go first
-constexpr int DEPTH = 4;
+constexpr int DEPTH = 2, SEEN = 8;
 
 DEV_INLINE unsigned to_bits(float x) {  // any NaN but ABSENT
   return x == x ? __builtin_bit_cast(unsigned, x) : 0x7fc00000u;
@@ -223,60 +240,69 @@ struct Chain {
 
   DEV_INLINE void publish(int slot, const Channel& ch, float A,
                           float C) const {
-    if (!ch.live) return;
     __hip_atomic_store(words + slot * BH + ch.state,
                        (uint64_t)to_bits(A) << 32 | to_bits(C),
                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 
   // The state before `slot`, found by one wave.
-  DEV_INLINE float look_back(int slot, const Channel& ch, float start) const {
-    float A = 1.f, C = 0.f;
-    bool met = !ch.live;
-    for (int back = slot - 1, polls = 0;;) {
+  DEV_INLINE float look_back(int slot, const Channel& ch, float start,
+                             Pair (*seen)[64]) const {
+    const uint64_t* own = words + (int64_t)slot * BH + ch.state;
+    float c = start;
+    int n = 0;  // slots before this one whose words are kept in `seen`
+    for (int polls = 0; n < slot;) {
       uint64_t p[DEPTH];
 #pragma unroll
       for (int q = 0; q < DEPTH; ++q)
-        p[q] = __hip_atomic_load(
-            words + (int64_t)max(back - q, 0) * BH + ch.state,
-            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      int seen = 0;
+        p[q] = __hip_atomic_load(own - min(n + 1 + q, slot) * BH,
+                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      bool met = false, more = true;
 #pragma unroll
       for (int q = 0; q < DEPTH; ++q) {
-        if (back - q < 0 || polls >= MOST_POLLS) {
-          const float c = back - q < 0 ? start : __builtin_nanf("");
-          return met ? C : A * c + C;
+        const unsigned bits = (unsigned)(p[q] >> 32);
+        const Pair r = {__builtin_bit_cast(float, bits),
+                        __builtin_bit_cast(float, (unsigned)p[q])};
+        if (!more || n == slot) continue;
+        if (__all(r.A < 0.f)) {
+          c = r.C;
+          met = true;
+          more = false;
+        } else if (n < SEEN && __all(bits != ABSENT)) {
+          seen[n++][lane_id()] = r;
+        } else {
+          more = false;
         }
-        if (!__all(met || (unsigned)(p[q] >> 32) != ABSENT)) break;
-        ++seen;
-        const float x = __builtin_bit_cast(float, (unsigned)(p[q] >> 32));
-        const float y = __builtin_bit_cast(float, (unsigned)p[q]);
-        C = met ? C : A * y + C;
-        A *= x;
-        met |= x < 0.f;
-        if (__all(met)) return C;
       }
-      back -= seen;
-      if (seen == 0) {
-        ++polls;
+      if (met) break;
+      if (!more) {
+        if (++polls == MOST_POLLS) {
+          c = __builtin_nanf("");
+          break;
+        }
         __builtin_amdgcn_s_sleep(1);
       }
     }
+    while (n > 0) {
+      const Pair r = seen[--n][lane_id()];
+      c = r.A < 0.f ? r.C : __builtin_fmaf(r.A, c, r.C);
+    }
+    return c;
   }
 
   // The state before `slot`, to all waves; the one behind it through `last`.
   // The waves that look back go first: the blocks behind wait for them.
   DEV_INLINE float hand_on(int slot, const Channel& ch, float A, float C,
-                           const float* start, float* lds, float* last,
+                           const float* start, float* lds, Pair (*seen)[64], float* last,
                            int w) const {
     if (w == 0) {
       __builtin_amdgcn_s_setprio(3);
       publish(slot, ch, A, C);
-      const float c = look_back(slot, ch, start ? start[ch.state] : 0.f);
+      const float c = look_back(slot, ch, start ? start[ch.state] : 0.f, seen);
       lds[lane_id()] = c;
-      const float behind = A * c + C;
+      const float behind = __builtin_fmaf(A, c, C);  // as look_back has it
       publish(slot, ch, -1.f, behind);
-      if (last && ch.live) last[ch.state] = behind;
+      if (last) last[ch.state] = behind;
       __builtin_amdgcn_s_setprio(0);
     }
     __syncthreads();
@@ -299,6 +325,7 @@ __global__ __launch_bounds__(64 * W) void glr_fwd_kernel(GlrArgs a) {
   __shared__ Pair lds[W][64];
   __shared__ float handed[64];
   __shared__ int taken;
+  __shared__ Pair seen[CHAIN ? SEEN : 1][64];
   const int waves = CHAIN ? W : blockDim.x / 64, lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
   const Slot slot =
@@ -309,9 +336,18 @@ __global__ __launch_bounds__(64 * W) void glr_fwd_kernel(GlrArgs a) {
   E* h0 = static_cast<E*>(a.h) + ch.first * a.h_b;
   const unsigned h_off = ch.offset<E>(a.h_b);
   const int t0 = (slot.order * waves + w) * K;
+  const int tiles = max(1, cdiv_const(ch.most, W * K));
+  if (CHAIN && slot.order >= tiles) {
+    E* h = h0 + (int64_t)t0 * a.h_t;
+    for (int t = t0; t < min(t0 + K, a.T); ++t, h += a.h_t)
+      at(h, h_off) = (E)0.f;
+    if (a.marks && t0 % GLR_MARK == 0 && t0 < a.T)
+      a.marks[(int64_t)(t0 / GLR_MARK) * a.B * a.H + ch.state] = 0.f;
+    return;
+  }
 
   Gates<E, K> g;
-  g.load(a, g0, ch.offset<E>(a.gates_b), t0);
+  g.load(a, g0, ch.offset<E>(a.gates_b), t0, max(ch.most, 1) - 1);
   g.mask(t0, ch.n_live);
   float x[K], y[K], A = 1.f, C = 0.f;
 #pragma unroll
@@ -332,24 +368,25 @@ __global__ __launch_bounds__(64 * W) void glr_fwd_kernel(GlrArgs a) {
         C = p.A * C + p.C;
         A *= p.A;
       }
-    c = Chain(a).hand_on(slot.order, ch, A, C, a.c0, handed,
-                         slot.order == a.chunks - 1 ? a.cT : nullptr, w);
+    c = Chain(a).hand_on(slot.order, ch, A, C, a.c0, handed, seen,
+                         slot.order == tiles - 1 ? a.cT : nullptr, w);
   } else {
     c = a.c0 ? a.c0[ch.state] : 0.f;
   }
   c = compose(c, lds, 0, w);
-  if (a.marks && t0 % GLR_MARK == 0 && t0 < a.T && ch.live)
+  if (a.marks && t0 % GLR_MARK == 0 && t0 < a.T)
     a.marks[(int64_t)(t0 / GLR_MARK) * a.B * a.H + ch.state] = c;
+  E* to = h0 + (int64_t)t0 * a.h_t;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int t = t0 + k;
     c = x[k] * c + y[k];
     const float h = sigmoid_tanh((float)g.o[k], c);
-    if (t < a.T && ch.live)
-      at(h0 + t * a.h_t, h_off) = t < ch.n_live ? (E)h : (E)0.f;
+    if (t < a.T) at(to, h_off) = t < ch.n_live ? (E)h : (E)0.f;
+    to += a.h_t;
   }
   // steps past T keep the state
-  if (!CHAIN && w == waves - 1 && ch.live) a.cT[ch.state] = c;
+  if (!CHAIN && w == waves - 1) a.cT[ch.state] = c;
 }
 
 // Tiles begin at marks; in a chain the first slot has the last of them.
@@ -360,6 +397,7 @@ __global__ __launch_bounds__(64 * W) void glr_bwd_kernel(GlrArgs a) {
   __shared__ Pair back[W][64];  // (A, D) of their gradients, last wave first
   __shared__ float handed[64];
   __shared__ int taken;
+  __shared__ Pair seen[CHAIN ? SEEN : 1][64];
   const int waves = CHAIN ? W : blockDim.x / 64, lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
   const int rw = waves - 1 - w;
@@ -372,15 +410,28 @@ __global__ __launch_bounds__(64 * W) void glr_bwd_kernel(GlrArgs a) {
   const unsigned dh_off = ch.offset<E>(a.dh_b);
   E* d0 = static_cast<E*>(a.dgates) + ch.first * a.dgates_b;
   const unsigned d_off = ch.offset<E>(a.dgates_b);
-  const int begin = CHAIN ? (a.chunks - 1 - slot.order) * W * K : 0;
+  const int tile = CHAIN ? a.chunks - 1 - slot.order : 0;
+  const int begin = tile * W * K;
   const int t0 = begin + w * K, stop = ch.n_live;
-
-  Gates<E, K> g;
-  g.load(a, g0, ch.offset<E>(a.gates_b), t0);
-  E dh[K];
+  const int tiles = max(1, cdiv_const(ch.most, W * K));
+  if (CHAIN && tile >= tiles) {
+    E* d = d0 + (int64_t)t0 * a.dgates_t;
+    for (int t = t0; t < min(t0 + K, a.T); ++t, d += a.dgates_t)
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-    dh[k] = at(dh0 + (int64_t)min(t0 + k, a.T - 1) * a.dh_t, dh_off);
+      for (int q = 0; q < 4; ++q) at(d + q * (int64_t)a.H, d_off) = (E)0.f;
+    return;
+  }
+
+  const int last = max(ch.most, 1) - 1;
+  Gates<E, K> g;
+  g.load(a, g0, ch.offset<E>(a.gates_b), t0, last);
+  E dh[K];
+  const E* from = dh0 + (int64_t)min(t0, last) * a.dh_t;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    dh[k] = at(from, dh_off);
+    from += t0 + k < last ? a.dh_t : 0;
+  }
   float c = a.marks[(int64_t)(begin / GLR_MARK) * a.B * a.H + ch.state];
   g.mask(t0, stop);
   if (!__all(t0 + K <= stop)) {
@@ -406,6 +457,7 @@ __global__ __launch_bounds__(64 * W) void glr_bwd_kernel(GlrArgs a) {
   // what the steps hand back from a gradient of zero behind them. The output
   // gate's gradient needs no more and is written at once.
   float before[K], u[K], D = 0.f;
+  E* d = d0 + (int64_t)t0 * a.dgates_t;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int t = t0 + k;
@@ -415,9 +467,10 @@ __global__ __launch_bounds__(64 * W) void glr_bwd_kernel(GlrArgs a) {
     const float o = sigmoid_f((float)g.o[k]);
     const float od = o * (float)dh[k];
     u[k] = od * (1.f - tc * tc);
-    if (t < a.T && ch.live)
-      at(d0 + t * a.dgates_t + 2 * (int64_t)a.H, d_off) =
+    if (t < a.T)
+      at(d + 2 * (int64_t)a.H, d_off) =
           t < stop ? (E)(od * tc * (1.f - o)) : (E)0.f;
+    d += a.dgates_t;
   }
 #pragma unroll
   for (int k = K - 1; k >= 0; --k) D = f[k] * (D + u[k]);
@@ -433,7 +486,7 @@ __global__ __launch_bounds__(64 * W) void glr_bwd_kernel(GlrArgs a) {
         sum = p.A * sum + p.C;
         whole *= p.A;
       }
-    carry = Chain(a).hand_on(slot.order, ch, whole, sum, a.dcT, handed,
+    carry = Chain(a).hand_on(tiles - 1 - tile, ch, whole, sum, a.dcT, handed, seen,
                              begin == 0 ? a.dc0 : nullptr, w);
   } else {
     carry = a.dcT ? a.dcT[ch.state] : 0.f;
@@ -444,16 +497,16 @@ __global__ __launch_bounds__(64 * W) void glr_bwd_kernel(GlrArgs a) {
     const int t = t0 + k;
     const float dc = carry + u[k], dci = dc * i[k], dcf = dc * f[k];
     carry = dcf;
-    if (t < a.T && ch.live) {
+    d -= a.dgates_t;
+    if (t < a.T) {
       const bool on = t < stop;
-      E* d = d0 + t * a.dgates_t;
       at(d, d_off) = on ? (E)(dci * n[k] * (1.f - i[k])) : (E)0.f;
       at(d + a.H, d_off) = on ? (E)(dcf * before[k] * (1.f - f[k])) : (E)0.f;
       at(d + 3 * (int64_t)a.H, d_off) =
           on ? (E)(dci * (1.f - n[k] * n[k])) : (E)0.f;
     }
   }
-  if (!CHAIN && w == 0 && ch.live) a.dc0[ch.state] = carry;
+  if (!CHAIN && w == 0) a.dc0[ch.state] = carry;
 }
 
 template <typename E>
