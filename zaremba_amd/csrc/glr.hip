@@ -291,19 +291,16 @@ struct Chain {
   }
 
   // The state before `slot`, to all waves; the one behind it through `last`.
-  // The waves that look back go first: the blocks behind wait for them.
   DEV_INLINE float hand_on(int slot, const Channel& ch, float A, float C,
                            const float* start, float* lds, Pair (*seen)[64], float* last,
                            int w) const {
     if (w == 0) {
-      __builtin_amdgcn_s_setprio(3);
       publish(slot, ch, A, C);
       const float c = look_back(slot, ch, start ? start[ch.state] : 0.f, seen);
       lds[lane_id()] = c;
       const float behind = __builtin_fmaf(A, c, C);  // as look_back has it
       publish(slot, ch, -1.f, behind);
       if (last) last[ch.state] = behind;
-      __builtin_amdgcn_s_setprio(0);
     }
     __syncthreads();
     return lds[lane_id()];
