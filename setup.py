@@ -4,6 +4,7 @@ The resulting zaremba_amd/_hip*.so travels with the repo snapshot to GPU
 boxes (no JIT cache involved). hipcc cross-compiles without a GPU.
 """
 
+import glob
 import os
 
 from setuptools import setup
@@ -13,6 +14,21 @@ os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
 from torch.utils.cpp_extension import BuildExtension, CUDAExtension  # noqa: E402
 
 here = os.path.dirname(os.path.abspath(__file__))
+
+
+def drop_stale_objects():
+    """The build knows of no header that a HIP source includes: an object
+    older than one of them would keep the old structs and constants, beside
+    objects that have the new ones. Such objects are compiled again."""
+    headers = glob.glob(os.path.join(here, "zaremba_amd/csrc/*.h"))
+    newest = max(map(os.path.getmtime, headers))
+    objects = os.path.join(here, "build/temp.*/**/*.o")
+    for path in glob.glob(objects, recursive=True):
+        if os.path.getmtime(path) < newest:
+            os.remove(path)
+
+
+drop_stale_objects()
 
 ext = CUDAExtension(
     name="zaremba_amd._hip",
