@@ -550,3 +550,20 @@ def test_a_tensor_of_over_two_to_the_31(bits):
     for u, v in zip(a, b):
         assert torch.equal(u, v)
     assert not bool(big["p"][:-k].any())
+
+
+@GPU
+def test_gradient_in_what_is_written():
+    x = make([10, 300], "cuda")
+    before = [p.clone() for p in x["params"]]
+    for grads in ([x["grads"][0], x["params"][1]],
+                  [x["exp_avgs"][1][:10], x["grads"][1]]):
+        with pytest.raises(RuntimeError, match="adamw"):
+            A.adamw_step_(x["params"], grads, x["exp_avgs"], x["exp_avg_sqs"],
+                          x["step"], lr=0.1)
+    assert all(torch.equal(a, b) for a, b in zip(x["params"], before))
+    # two parameters may have one gradient
+    one = torch.cat([x["grads"][1], x["grads"][0]])
+    A.adamw_step_(x["params"], [one[:10], one[:300]], x["exp_avgs"],
+                  x["exp_avg_sqs"], x["step"], lr=0.1)
+    assert not any(torch.equal(a, b) for a, b in zip(x["params"], before))

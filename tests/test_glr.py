@@ -565,3 +565,49 @@ def test_rows_that_end_at_tiles(H, ends):
     gates = gates.masked_fill(~live, float("nan"))
     dh = dh.masked_fill(~live, float("nan"))
     check(gates, c0, dh, dcT, lengths)
+
+
+@GPU
+def test_refusals_of_shared_memory_and_sizes():
+    T, B, H = 8, 3, 4
+    gates, c0, dh, dcT, _ = make(T, B, H, torch.float32, "cuda")
+    _, _, marks = G.glr_forward(gates, c0, training=True)
+    room = torch.zeros(T * B * 4 * H, device="cuda")
+    h = room[:T * B * H].view(T, B, H)
+    d = room.view(T, B, 4 * H)
+    state = room[-B * H:].view(B, H)
+    in_h = h.view(-1)[5:5 + B * H].view(B, H)
+    lengths = room[4:4 + B].view(torch.int32)
+    grad = torch.zeros(T, B, H, device="cuda", requires_grad=True)
+    # 2^31 channels of one step would do, but not in 9: no such tensor is made
+    wide = torch.empty(1, 1, 4 * 32767, device="cuda").expand(9, 65536, -1)
+    for call in (
+            lambda: G.glr_forward(gates, in_h, out=h),
+            lambda: G.glr_forward(gates, c0, lengths, out=h),
+            lambda: G.glr_forward(gates, c0, out=grad),
+            lambda: G.glr_backward(dh, state, gates, c0, marks, out=d),
+            lambda: G.glr_backward(dh, dcT, gates, c0, marks, lengths, out=d),
+            lambda: G.glr_backward(h, dcT, gates, c0, marks, out=d),
+            lambda: G.glr_backward(
+                dh, dcT, gates, c0, room[:marks.numel()].view(marks.shape),
+                out=d),
+            lambda: G.glr_forward(wide)):
+        with pytest.raises(RuntimeError, match="glr"):
+            call()
+    assert not room.any()
+    want = G.glr_forward(gates, c0)[0]
+    assert torch.equal(G.glr_forward(gates, c0, out=h)[0], want)
+    with torch.no_grad():
+        G.glr_forward(gates, c0, out=grad)
+    assert torch.equal(grad.detach(), want)
+
+
+@GPU
+def test_step_in_inference_mode():
+    gates, c0, *_ = make(1, 3, 70, torch.float32, "cuda")
+    c = c0.clone()
+    want = G.glr_step(gates[0], c)
+    with torch.inference_mode():
+        state = c0.clone()
+        assert torch.equal(G.glr_step(gates[0], state), want)
+        assert torch.equal(state, c)

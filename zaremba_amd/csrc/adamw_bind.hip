@@ -134,6 +134,17 @@ OptTensor adamw_step_(const Tensors& params, const Tensors& grads,
   for (size_t k = 1; k < written.size(); ++k)
     TORCH_CHECK(written[k - 1].second <= written[k].first,
                 "adamw_step_: parameters, states or shadows share memory");
+  // other blocks read a gradient while these are written
+  for (size_t k = 0; k < count; ++k) {
+    const char* at = static_cast<const char*>(grads[k].data_ptr());
+    const auto next = std::upper_bound(
+        written.begin(), written.end(), at,
+        [](const char* x, const auto& range) { return x < range.second; });
+    TORCH_CHECK(next == written.end() ||
+                next->first >= at + grads[k].nbytes(),
+                "adamw_step_: grads[", k, "] shares memory with what the "
+                "step writes");
+  }
 
   int64_t total = 0;
   for (const auto& t : all) total += t.n;

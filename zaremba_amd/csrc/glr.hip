@@ -552,13 +552,24 @@ int rows_per_launch(const GlrArgs& a, int size) {
   return (apart * most + 4 * (int64_t)a.H) * size < (int64_t)1 << 32 ? a.B : 1;
 }
 
+// Tiles of a chain; 0 where one tile is the window.
+int chunks_of(int64_t T, bool back) {
+  return T > MIDDLE_STEPS * TILE_WAVES
+             ? cdiv(T, (back ? BWD_STEPS : FWD_STEPS) * CHAIN_WAVES)
+             : 0;
+}
+
 GlrArgs planned(GlrArgs a, bool back, int size) {
   a.rows = rows_per_launch(a, size);
   a.groups = cdiv((int64_t)a.rows * a.H, 64);
-  a.chunks = a.T > MIDDLE_STEPS * TILE_WAVES
-                 ? cdiv(a.T, (back ? BWD_STEPS : FWD_STEPS) * CHAIN_WAVES)
-                 : 0;
+  a.chunks = chunks_of(a.T, back);
   return a;
+}
+
+// At least as many for each counter as it has slots.
+int64_t chain_blocks(int64_t groups, int64_t chunks) {
+  return groups >= SHARED_FROM ? (int64_t)XCDS * cdiv(groups, XCDS) * chunks
+                               : (int64_t)XCDS * cdiv(chunks, XCDS) * groups;
 }
 
 template <bool BACK, typename E>
@@ -571,10 +582,7 @@ void launch(const GlrArgs& args, hipStream_t stream) {
                          stream, reinterpret_cast<uint4*>(a.work), n);
       auto kernel = BACK ? glr_bwd_kernel<E, BWD_STEPS, CHAIN_WAVES, true>
                          : glr_fwd_kernel<E, FWD_STEPS, CHAIN_WAVES, true>;
-      const int blocks =
-          a.groups >= SHARED_FROM ? XCDS * cdiv(a.groups, XCDS) * a.chunks
-                                  : XCDS * cdiv(a.chunks, XCDS) * a.groups;
-      hipLaunchKernelGGL(kernel, dim3(blocks),
+      hipLaunchKernelGGL(kernel, dim3(chain_blocks(a.groups, a.chunks)),
                          dim3(64 * CHAIN_WAVES), 0, stream, a);
     } else if (a.T <= SHORT_STEPS * TILE_WAVES) {
       auto kernel = BACK ? glr_bwd_kernel<E, SHORT_STEPS, TILE_WAVES, false>
@@ -597,6 +605,13 @@ int64_t glr_work_words(const GlrArgs& args, bool back, int size) {
   if (!a.chunks) return 0;
   const int64_t n = COUNTER_WORDS + (int64_t)a.chunks * a.B * a.H;
   return n + (n & 1);
+}
+
+int64_t glr_threads(int64_t T, int64_t B, int64_t H, bool back) {
+  const int64_t groups = cdiv(B * H, 64), chunks = chunks_of(T, back);
+  if (chunks) return chain_blocks(groups, chunks) * 64 * CHAIN_WAVES;
+  return groups * 64 *
+         cdiv(T, T <= SHORT_STEPS * TILE_WAVES ? SHORT_STEPS : MIDDLE_STEPS);
 }
 
 void launch_glr_fwd(const GlrArgs& a, GlrType type, hipStream_t stream) {

@@ -30,7 +30,8 @@ GlrType glr_type(const Tensor& t, const char* op) {
   }
 }
 
-void check_gates(const Tensor& gates, int64_t dims, const char* op) {
+void check_gates(const Tensor& gates, int64_t dims, const char* op,
+                 bool back = false) {
   TORCH_CHECK(gates.is_cuda(), op, ": gates must be on the GPU");
   TORCH_CHECK(gates.dim() == dims, op, ": gates must be ",
               dims == 3 ? "[T, B, 4H]" : "[B, 4H]", ", got ", gates.sizes());
@@ -39,7 +40,9 @@ void check_gates(const Tensor& gates, int64_t dims, const char* op) {
               gates.size(-1), " values");
   const int64_t B = gates.size(-2), H = gates.size(-1) / 4;
   TORCH_CHECK(B * H < std::numeric_limits<int>::max() - 64 &&
-              (dims == 2 || gates.size(0) < std::numeric_limits<int>::max()),
+              (dims == 2 ||
+               (gates.size(0) < std::numeric_limits<int>::max() &&
+                glr_threads(gates.size(0), B, H, back) < (int64_t)1 << 32)),
               op, ": sizes ", gates.sizes(), " are too large");
 }
 
@@ -87,6 +90,13 @@ bool overlap(const Tensor& a, const Tensor& b) {
   return x.first < y.second && y.first < x.second;
 }
 
+// What is read while `out` is written.
+void check_apart(const Tensor& out, const Tensor& x, const char* name,
+                 const char* op) {
+  TORCH_CHECK(!x.defined() || !overlap(out, x), op,
+              ": out shares memory with ", name);
+}
+
 void check_out(const Tensor& out, const Tensor& gates, int64_t width,
                const char* op) {
   TORCH_CHECK(out.scalar_type() == gates.scalar_type() &&
@@ -95,7 +105,9 @@ void check_out(const Tensor& out, const Tensor& gates, int64_t width,
               out.size(2) == width && out.is_contiguous(),
               op, ": out must be a contiguous [", gates.size(0), ", ",
               gates.size(1), ", ", width, "] of the gates' type and device");
-  TORCH_CHECK(!overlap(out, gates), op, ": out shares memory with gates");
+  TORCH_CHECK(!at::GradMode::is_enabled() || !out.requires_grad(), op,
+              ": out requires a gradient, which this call does not record");
+  check_apart(out, gates, "gates", op);
 }
 
 Tensor dense_rows(const Tensor& t) {
@@ -151,6 +163,8 @@ std::tuple<Tensor, Tensor, OptTensor> glr_forward(
   if (out) {
     h = *out;
     check_out(h, gates, a.H, op);
+    check_apart(h, c0, "c0", op);
+    check_apart(h, keep, "lengths", op);
     h.unsafeGetTensorImpl()->bump_version();
   } else {
     h = empty_as(gates, a.H);
@@ -180,7 +194,7 @@ std::tuple<Tensor, Tensor> glr_backward(
     const OptTensor& c0_in, const Tensor& marks, const OptTensor& lengths,
     const OptTensor& out) {
   const char* op = "glr_backward";
-  check_gates(gates_in, 3, op);
+  check_gates(gates_in, 3, op, true);
   const GlrType type = glr_type(gates_in, op);
   c10::DeviceGuard guard(gates_in.device());
   const Tensor gates = dense_rows(gates_in);
@@ -220,7 +234,10 @@ std::tuple<Tensor, Tensor> glr_backward(
   if (out) {
     dgates = *out;
     check_out(dgates, gates, 4 * (int64_t)a.H, op);
-    TORCH_CHECK(!overlap(dgates, dh), op, ": out shares memory with dh");
+    check_apart(dgates, dh, "dh", op);
+    check_apart(dgates, dcT, "dcT", op);
+    check_apart(dgates, marks, "marks", op);
+    check_apart(dgates, keep, "lengths", op);
     dgates.unsafeGetTensorImpl()->bump_version();
   } else {
     dgates = empty_as(gates, 4 * (int64_t)a.H);

@@ -104,6 +104,8 @@ struct GlrArgs {
 };
 // Words of 64 bits that a call needs for itself; size: of a gate in bytes.
 int64_t glr_work_words(const GlrArgs& a, bool back, int size);
+// Threads of the largest launch for these sizes: a grid has fewer than 2^32.
+int64_t glr_threads(int64_t T, int64_t B, int64_t H, bool back);
 void launch_glr_fwd(const GlrArgs& a, GlrType type, hipStream_t stream);
 void launch_glr_bwd(const GlrArgs& a, GlrType type, hipStream_t stream);
 void launch_glr_step(const GlrArgs& a, GlrType type, hipStream_t stream);
