@@ -1,7 +1,7 @@
 #!/bin/bash
 # Round-2 GPU session 2: full gpu pytest (fixed RCCL skip + ksplit
 # parity + softmax_acc), bwd census 2-way vs 4-way K-split, bench A/B,
-# then the CPX partition probe for real-RCCL DP evidence.
+# K-split parity evidence.
 set -x
 mkdir -p gpurun_out
 cd /root/repo
@@ -18,9 +18,7 @@ ZAREMBA_AMD_BWD_KSPLIT=4 timeout 300 python bench.py --gpus 1 --steps 60 --warmu
   > gpurun_out/s2_bench_ks4.json 2>gpurun_out/s2_bench_ks4.err
 echo "ks4 bench rc=$?" >> gpurun_out/s2_bench_ks4.err
 
-bash tools/gpu_cpx_dp.sh > gpurun_out/s2_cpx.out 2>&1
 
 tail -n 16 gpurun_out/s2_census_ks2.txt gpurun_out/s2_census_ks4.txt
 cat gpurun_out/s2_bench_ks2.json gpurun_out/s2_bench_ks4.json
 tail -n 6 gpurun_out/s2_pytest.log
-tail -n 25 gpurun_out/cpx_dp.log
