@@ -13,11 +13,12 @@
 // is never rounded to zero, so that no update divides by eps alone.
 //
 // Two launches: the sum of squares (the norm is of all gradients, so they are
-// read twice), and the update, in which each block first adds up the partial
-// sums while its first loads are in flight. At 66.0M parameters with bf16
-// shadows they take 427 us in 32 bits (2.25 GB with the second reading, 5.26
-// TB/s, what a copy reaches), and 300 us in 8 bits (1.45 GB, 4.8 TB/s), where
-// vector instructions, some 86 a value, are busy 85 % of the update's time.
+// read twice), and the update, in which a wave of each block first adds up the
+// partial sums while all of the block's loads are in flight. At 66.0M
+// parameters with bf16 shadows they take 416 us in 32 bits (2.25 GB with the
+// second reading, 5.4 TB/s, more than the 5.2 of a copy as a cache holds some of
+// it), and 279 us in 8 bits (1.46 GB, 5.2 TB/s; some 62 vector instructions a
+// value).
 //
 // Sums and the arithmetic of an update are in the order of the formulas, each
 // product and sum rounded (no contraction), and the norm is summed in 64 bits
@@ -154,19 +155,32 @@ __global__ __launch_bounds__(THREADS) void adamw_norm_kernel(
 }
 
 // What the gradients are multiplied by: in every block the same sum, in the
-// same order.
+// same order, by one wave, as the root and the quotient in 64 bits cost as
+// much as some 100 values.
 DEV_INLINE float clip_scale(const AdamwScalars& s, const AdamwWork& w,
                             bool tell) {
-  __shared__ double lds[WAVES];
+  __shared__ float scale;
   if (!s.clip) return (float)s.grad_scale;
-  double sum = 0;
-  for (int i = threadIdx.x; i < w.count; i += THREADS) sum += w.partials[i];
-  sum = block_sum(sum, lds);
-  const double norm = __builtin_sqrt(sum) * s.grad_scale;
-  if (tell && threadIdx.x == 0) *w.norm = (float)norm;
-  double coef = s.max_norm / (norm + 1e-6);
-  if (coef > 1) coef = 1;  // a norm that is NaN stays one
-  return (float)(coef * s.grad_scale);
+  if (wave_id() == 0) {
+    constexpr int R = 8;  // loads in flight
+    double sum = 0;
+    for (int i = lane_id(); i < w.count; i += 64 * R) {
+      double x[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        x[r] = w.partials[min(i + 64 * r, w.count - 1)];
+#pragma unroll
+      for (int r = 0; r < R; ++r) sum += i + 64 * r < w.count ? x[r] : 0.;
+    }
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    const double norm = __builtin_sqrt(sum) * s.grad_scale;
+    if (tell && threadIdx.x == 0) *w.norm = (float)norm;
+    double coef = s.max_norm / (norm + 1e-6);
+    if (coef > 1) coef = 1;  // a norm that is NaN stays one
+    scale = (float)(coef * s.grad_scale);
+  }
+  __syncthreads();
+  return scale;
 }
 
 constexpr unsigned HASH_INDEX = 0x9E3779B1u, HASH_STEP = 0x85EBCA77u;
@@ -194,19 +208,46 @@ DEV_INLINE float sqrt_f(float x) {
   return __builtin_fmaf(-up, s, x) > 0.f ? up : r;
 }
 
-// One of the two codes beside x (0 <= x), so that x^2 is right in the mean.
-// hashed: step * C2 + index * C1 of the element.
-DEV_INLINE unsigned draw_e4m3(float x, unsigned hashed) {
-  // less than the least code is drawn as the least code; 0 is put back below
-  const float y = __builtin_fminf(__builtin_fmaxf(x, 0x1p-9f), E4M3_MAX);
-  unsigned low = (__builtin_bit_cast(unsigned, y) >> 20) - 960u;
-  low = y < 0x1p-6f ? (unsigned)(y * 512.f) : low;
+// Of y's nearest code and one of its neighbours, those on either side of y:
+// the one below, or, as a draw has it, the one above, so that y^2 is right in
+// the mean. hashed: step * C2 + index * C1 of the element.
+DEV_INLINE unsigned draw_e4m3(float y, unsigned nearest, float value,
+                              unsigned hashed) {
+  unsigned low = nearest - (value > y);
   const f32x2 ab =
       __builtin_amdgcn_cvt_pk_f32_fp8((int)(low * 257u + 256u), false);
   const float aa = ab.x * ab.x;
   // above 126 is a NaN, and no number less than one
   low += hash_uniform(hashed) * (ab.y * ab.y - aa) < y * y - aa;
-  return x > 0.f ? low : 0;
+  return low;
+}
+
+// The codes of four x >= 0. Less than the least code is drawn as the least
+// code; 0 stays 0.
+DEV_INLINE unsigned draw4_e4m3(const float (&x)[4], unsigned hashed) {
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    y[e] = __builtin_fminf(__builtin_fmaxf(x[e], 0x1p-9f), E4M3_MAX);
+  int near = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  near = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], near, true);
+  unsigned codes =
+      draw_e4m3(y[0], near & 255, __builtin_amdgcn_cvt_f32_fp8(near, 0),
+                hashed) |
+      draw_e4m3(y[1], near >> 8 & 255, __builtin_amdgcn_cvt_f32_fp8(near, 1),
+                hashed + HASH_INDEX) << 8 |
+      draw_e4m3(y[2], near >> 16 & 255, __builtin_amdgcn_cvt_f32_fp8(near, 2),
+                hashed + 2 * HASH_INDEX) << 16 |
+      draw_e4m3(y[3], (unsigned)near >> 24,
+                __builtin_amdgcn_cvt_f32_fp8(near, 3),
+                hashed + 3 * HASH_INDEX) << 24;
+  const float least =
+      __builtin_fminf(__builtin_fminf(x[0], x[1]), __builtin_fminf(x[2], x[3]));
+  if (!(least > 0.f))
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (!(x[e] > 0.f)) codes &= ~(255u << 8 * e);
+  return codes;
 }
 
 // The largest of a wave, in every lane.
@@ -330,7 +371,7 @@ struct Block {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         um = max(um, magnitude(m1.v[e]));
-        ur = max(ur, magnitude(r1.v[e]));
+        ur = max(ur, __builtin_bit_cast(unsigned, r1.v[e]));
       }
       // half the wave divides for m, half for r
       const unsigned am = wave_max(um), ar = wave_max(ur);
@@ -348,10 +389,9 @@ struct Block {
                                           true);
       __builtin_memcpy(&m, &c, 4);
       const unsigned hashed = x.hashed + i * HASH_INDEX;
-      unsigned codes = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        codes |= draw_e4m3(r1.v[e] * ir, hashed + e * HASH_INDEX) << 8 * e;
+      const float x4[4] = {r1.v[0] * ir, r1.v[1] * ir, r1.v[2] * ir,
+                           r1.v[3] * ir};
+      const unsigned codes = draw4_e4m3(x4, hashed);
       __builtin_memcpy(&v, &codes, 4);
     }
     if (WHOLE) {
@@ -379,8 +419,8 @@ struct Block {
 template <typename G, bool BITS8>
 __global__ __launch_bounds__(THREADS) void adamw_update_kernel(
     AdamwTensors a, AdamwScalars s, bool tell, AdamwWork w) {
-  constexpr int AHEAD = 2;  // blocks of 256 that a wave has in flight
   constexpr int STRIDE = WAVES * QBLOCK;
+  constexpr int EACH = ADAMW_CHUNK / STRIDE;  // blocks of 256 of a wave
   // From the last chunk to the first: the gradients that the norm read last
   // are those that a cache may still hold.
   const int c = a.begin[a.count] - 1 - (int)blockIdx.x;
@@ -391,24 +431,20 @@ __global__ __launch_bounds__(THREADS) void adamw_update_kernel(
   const int whole = n / QBLOCK * QBLOCK;
   const int wave = __builtin_amdgcn_readfirstlane(wave_id());
 
-  int q = wave * QBLOCK;
-  Block<G, BITS8> b[AHEAD];
+  Block<G, BITS8> b[EACH];
 #pragma unroll
-  for (int r = 0; r < AHEAD; ++r)
-    if (q + r * STRIDE < whole)
-      b[r].template load<true>(x, q + r * STRIDE, 4);
+  for (int r = 0; r < EACH; ++r) {
+    const int q = wave * QBLOCK + r * STRIDE;
+    if (q < whole) b[r].template load<true>(x, q, 4);
+  }
   const float coef = clip_scale(s, w, tell && blockIdx.x == 0);
   const float rate = w.values->rate, root = w.values->root;
   x.hashed += w.values->step * HASH_STEP;
-  for (; q < whole; q += AHEAD * STRIDE) {
 #pragma unroll
-    for (int r = 0; r < AHEAD; ++r) {
-      const int i = q + r * STRIDE;
-      if (i >= whole) break;
-      b[r].template update<true>(x, i, 4, s, coef, rate, root);
-      if (i + AHEAD * STRIDE < whole)
-        b[r].template load<true>(x, i + AHEAD * STRIDE, 4);
-    }
+  for (int r = 0; r < EACH; ++r) {
+    const int q = wave * QBLOCK + r * STRIDE;
+    if (q < whole)
+      b[r].template update<true>(x, q, 4, s, coef, rate, root);
   }
   // what is left of the tensor behind its last whole 256
   if (whole < n && wave == whole / QBLOCK % WAVES) {
@@ -421,10 +457,10 @@ __global__ __launch_bounds__(THREADS) void adamw_update_kernel(
 
 }  // namespace
 
-// Every block of the update reads the partial sums of all of these: 512 to
-// 1536 measured the same, 4096 8 % more at 66M parameters in 8 bits.
+// Every block of the update reads the partial sums of all of these: at 66M
+// parameters in 8 bits 512 take 285 us, 1024 290 and 256 286.
 int adamw_norm_blocks(const AdamwTensors& a, int launches) {
-  return std::max(1, std::min(a.norm_begin[a.count], 1024 / launches));
+  return std::max(1, std::min(a.norm_begin[a.count], 512 / launches));
 }
 
 void launch_adamw_norm(const AdamwTensors& a, const AdamwScalars& s,

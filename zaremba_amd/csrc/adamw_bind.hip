@@ -5,7 +5,6 @@
 #include <c10/core/DeviceGuard.h>
 
 #include <algorithm>
-#include <limits>
 #include <string>
 #include <utility>
 #include <vector>
@@ -148,7 +147,8 @@ OptTensor adamw_step_(const Tensors& params, const Tensors& grads,
 
   int64_t total = 0;
   for (const auto& t : all) total += t.n;
-  TORCH_CHECK(total / ADAMW_NORM_CHUNK < std::numeric_limits<int>::max() / 8,
+  // a grid has fewer than 2^32 threads, 256 a block
+  TORCH_CHECK(total / ADAMW_CHUNK + (int64_t)count < 1 << 24,
               "adamw_step_: too many values");
   AdamwScalars s = {};
   s.step = step.data_ptr<int64_t>();

@@ -114,7 +114,10 @@ void launch_glr_step(const GlrArgs& a, GlrType type, hipStream_t stream);
 // arguments (4 KB at most), so that no call copies a table to the device.
 constexpr int ADAMW_TENSORS = 48;
 constexpr int ADAMW_NORM_CHUNK = 8192;  // values of a tensor at a time
-constexpr int ADAMW_CHUNK = 4096;       // values of a block, of one tensor
+// Values of a block of the update, of one tensor. At 66M parameters 1024, 2048
+// and 4096 take 408, 416 and 422 us in 32 bits and 299, 279 and 285 in 8; at
+// 4.7M 31, 29.6 and 29.6.
+constexpr int ADAMW_CHUNK = 2048;
 struct AdamwTensor {
   float* p;
   const void* g;       // f32 or bf16
