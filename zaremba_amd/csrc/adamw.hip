@@ -353,7 +353,7 @@ struct Block {
       }
       m1.v[e] = m0 * s.b1 + gr * s.c1;
       const float v1 = v0 * s.b2 + gr * gr * s.c2;
-      // In 8 bits the arithmetic is what bounds the kernel: one reciprocal,
+      // In 8 bits the arithmetic takes over half of the time: one reciprocal,
       // off by one unit of 2^-23, in place of a division's dozen of steps.
       r1.v[e] = BITS8 ? sqrt_f(v1) : __builtin_sqrtf(v1);
       const float d = r1.v[e] * root + s.eps;
