@@ -179,6 +179,65 @@ def rel(a, b):
 SCORES, GRADS = 1e-2, 2e-2
 
 
+def _grads_of(m, seed, states):
+    x, y = batch(5, 3, 60, seed=seed)
+    scores, states = m(x, [(h.detach(), c.detach()) for h, c in states])
+    F_ref.nll_loss(scores, y).backward()
+    return states
+
+
+def _rank_main(rank, world, init_file, bits, q):
+    import torch.distributed as td
+    from zaremba_amd.parallel.bucketer import GradBucketer
+    torch.set_num_threads(1)
+    td.init_process_group("gloo", init_method=f"file://{init_file}",
+                          rank=rank, world_size=world)
+    m = model()
+    dp = GradBucketer(m, bucket_bytes=4096)
+    opt, states = AdamW(m.parameters(), bits=bits), m.state_init(3)
+    for step in range(3):
+        dp.zero_grad()
+        states = _grads_of(m, 10 * step + rank, states)
+        dp.finalize_backward()
+        trainer.adamw_step(m, opt, 1e-2, 0.5)
+    q.put((rank, [p.detach().numpy().copy() for p in m.parameters()]))
+    td.destroy_process_group()
+
+
+@pytest.mark.timeout(180)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_ranks_step_alike(tmp_path, bits):
+    """Two ranks with a batch each stay one model: the one that takes both
+    batches. A sum of two gradients has one rounding in either order."""
+    import torch.multiprocessing as mp
+    ctx = mp.get_context("spawn")
+    q = ctx.SimpleQueue()
+    procs = [ctx.Process(target=_rank_main, args=(
+        r, 2, str(tmp_path / "pg"), bits, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict(q.get() for _ in procs)
+    for p in procs:
+        p.join(60)
+        assert p.exitcode == 0
+    threads = torch.get_num_threads()
+    torch.set_num_threads(1)
+    try:
+        m = model()
+        opt = AdamW(m.parameters(), bits=bits)
+        states = [m.state_init(3) for _ in range(2)]
+        for step in range(3):
+            m.zero_grad()
+            states = [_grads_of(m, 10 * step + r, states[r])
+                      for r in range(2)]
+            trainer.adamw_step(m, opt, 1e-2, 0.5)
+    finally:
+        torch.set_num_threads(threads)
+    for a, b, p in zip(got[0], got[1], m.parameters()):
+        assert torch.equal(torch.from_numpy(a), torch.from_numpy(b))
+        assert torch.equal(torch.from_numpy(a), p.detach())
+
+
 @GPU
 @pytest.mark.parametrize("T,B,H", [(35, 20, 200), (9, 40, 64), (700, 2, 72)])
 def test_hip_model_follows_eager(T, B, H):
