@@ -611,3 +611,20 @@ def test_step_in_inference_mode():
         state = c0.clone()
         assert torch.equal(G.glr_step(gates[0], state), want)
         assert torch.equal(state, c)
+
+
+@GPU
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,B,H", [(129, 17, 1001), (300, 33, 500),
+                                   (450, 16, 1024)])
+def test_windows_of_many_channels(T, B, H, dtype):
+    """Over 128 steps of over 16384 channels, in shorter tiles: whole rows
+    and rows that end anywhere, twice with the same bits."""
+    for ragged in (False, True):
+        gates, c0, dh, dcT, lengths = make(T, B, H, dtype, "cuda",
+                                           ragged=ragged)
+        h, cT, dgates, dc0 = check(gates, c0, dh, dcT, lengths)
+        again = G.glr_forward(gates, c0, lengths, training=True)
+        assert torch.equal(again[0], h) and torch.equal(again[1], cT)
+        back = G.glr_backward(dh, dcT, gates, c0, again[2], lengths)
+        assert torch.equal(back[0], dgates) and torch.equal(back[1], dc0)

@@ -169,9 +169,9 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 //
 // A tile behind the last step of each of its rows writes zeros and ends; the
 // chain ends, or in the backward pass begins, with the tile before. Rows of
-// random lengths, forward / backward: 133 / 243 us against 155 / 279 with such
-// tiles in the chain at 512 x 80 x 1500, 28 / 55 against 35 / 59 at 1001 x 17 x
-// 651. Their reads are half of all; an XCD whose rows are short then waits for
+// random lengths, forward / backward in tiles of 8 waves: 133 / 243 us against
+// 155 / 279 with such tiles in the chain at 512 x 80 x 1500, 28 / 55 against
+// 35 / 59 at 1001 x 17 x 651. Their reads are half of all; an XCD whose rows are short then waits for
 // the others, and dealing groups out in smaller pieces costs as much in lines
 // that two XCDs read.
 //
@@ -185,11 +185,11 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 // seldom whole cache lines, and the other halves are then met in the same L2.
 // With fewer groups each has a counter of its own, as the blocks of one would
 // queue at one address (14 ns a slot) and an XCD would have 3 groups or less.
-// Measured in us, forward / backward, bf16, H = 1500: with a counter a group
-// against shares, 23.4 groups x 65536 steps 250 / 537 against 276 / 578 (one
-// counter for all: 260 / 545), 15.6 x 16384 (H = 1000) 53 / 90 against 52 / 99,
-// but 94 x 4096 69 / 141 against 65 / 120 and 375 x 1024 70 / 146 against 62 /
-// 113.
+// Measured in us, forward / backward in tiles of 8 waves, bf16, H = 1500: with
+// a counter a group against shares, 23.4 groups x 65536 steps 250 / 537 against
+// 276 / 578 (one counter for all: 260 / 545), 15.6 x 16384 (H = 1000) 53 / 90
+// against 52 / 99, but 94 x 4096 69 / 141 against 65 / 120 and 375 x 1024 70 /
+// 146 against 62 / 113.
 //
 // At T = 65536, B = 1, H = 1500, bf16 this takes 250 us forward (983 MB, 3.9
 // TB/s of the 5.2 that a copy reaches) and 537 backward (1770 MB, 3.3 TB/s);
@@ -535,12 +535,18 @@ void by_type(GlrType type, F f) {
 // 128 one of waves with 8. A chain's tiles are 128 steps forward, 64 backward,
 // of 8 waves. 16 waves with 8 steps measured 218 us against 200 forward at
 // 65536 x 1 x 1472, 4 waves with 16 566 against 545 backward at 65536 x 1 x
-// 1500. Blocks that loop over tiles, which need no chain, measured the same up to 128 steps, and from 256 steps
+// 1500. Forward with MANY_GROUPS, a group for each CU, tiles are 64 steps of 4
+// waves: blocks end sooner, and more of them wait while others load. 300 x 64 x
+// 650 takes 34 us against 39, 512 x 80 x 1500 135 against 147 and with random
+// lengths 110 against 127, 1024 x 16 x 1500 56 against 60, but 256 x 20 x 1500
+// 21.8 against 21.3; with fewer groups 65536 x 1 x 1500 273 against 256, 8192 x 2
+// x 1024 f32 73 against 70. Backward the same costs 3 to 15 %. Blocks that loop over tiles, which need no chain, measured the same up to 128 steps, and from 256 steps
 // on up to four times a chain's time where channels are few (23 groups, 512
 // steps: 20 / 33 us against 10 / 14) and 1.1 to 1.4 times where they are many
 // (1875 groups, 512 steps: 161 / 401 against 153 / 292).
 constexpr int SHORT_STEPS = 4, MIDDLE_STEPS = 8, TILE_WAVES = 16;
 constexpr int FWD_STEPS = 16, BWD_STEPS = 8, CHAIN_WAVES = 8;
+constexpr int MANY_GROUPS = 256, MANY_WAVES = 4;
 
 // Rows of one launch: all, unless rows lie so far apart that those of a block
 // do not fit a lane's 32-bit offset; then one.
@@ -552,17 +558,22 @@ int rows_per_launch(const GlrArgs& a, int size) {
   return (apart * most + 4 * (int64_t)a.H) * size < (int64_t)1 << 32 ? a.B : 1;
 }
 
+int chain_waves(int64_t groups, bool back) {
+  return back || groups < MANY_GROUPS ? CHAIN_WAVES : MANY_WAVES;
+}
+
 // Tiles of a chain; 0 where one tile is the window.
-int chunks_of(int64_t T, bool back) {
+int chunks_of(int64_t T, int64_t groups, bool back) {
   return T > MIDDLE_STEPS * TILE_WAVES
-             ? cdiv(T, (back ? BWD_STEPS : FWD_STEPS) * CHAIN_WAVES)
+             ? cdiv(T, (back ? BWD_STEPS : FWD_STEPS) *
+                           chain_waves(groups, back))
              : 0;
 }
 
 GlrArgs planned(GlrArgs a, bool back, int size) {
   a.rows = rows_per_launch(a, size);
   a.groups = cdiv((int64_t)a.rows * a.H, 64);
-  a.chunks = chunks_of(a.T, back);
+  a.chunks = chunks_of(a.T, a.groups, back);
   return a;
 }
 
@@ -580,10 +591,13 @@ void launch(const GlrArgs& args, hipStream_t stream) {
       const int64_t n = glr_work_words(args, BACK, sizeof(E)) / 2;
       hipLaunchKernelGGL(glr_reset_kernel, dim3(cdiv(n, 256)), dim3(256), 0,
                          stream, reinterpret_cast<uint4*>(a.work), n);
+      const int waves = chain_waves(a.groups, BACK);
       auto kernel = BACK ? glr_bwd_kernel<E, BWD_STEPS, CHAIN_WAVES, true>
-                         : glr_fwd_kernel<E, FWD_STEPS, CHAIN_WAVES, true>;
+                    : waves == CHAIN_WAVES
+                        ? glr_fwd_kernel<E, FWD_STEPS, CHAIN_WAVES, true>
+                        : glr_fwd_kernel<E, FWD_STEPS, MANY_WAVES, true>;
       hipLaunchKernelGGL(kernel, dim3(chain_blocks(a.groups, a.chunks)),
-                         dim3(64 * CHAIN_WAVES), 0, stream, a);
+                         dim3(64 * waves), 0, stream, a);
     } else if (a.T <= SHORT_STEPS * TILE_WAVES) {
       auto kernel = BACK ? glr_bwd_kernel<E, SHORT_STEPS, TILE_WAVES, false>
                          : glr_fwd_kernel<E, SHORT_STEPS, TILE_WAVES, false>;
@@ -608,8 +622,9 @@ int64_t glr_work_words(const GlrArgs& args, bool back, int size) {
 }
 
 int64_t glr_threads(int64_t T, int64_t B, int64_t H, bool back) {
-  const int64_t groups = cdiv(B * H, 64), chunks = chunks_of(T, back);
-  if (chunks) return chain_blocks(groups, chunks) * 64 * CHAIN_WAVES;
+  const int64_t groups = cdiv(B * H, 64), chunks = chunks_of(T, groups, back);
+  if (chunks)
+    return chain_blocks(groups, chunks) * 64 * chain_waves(groups, back);
   return groups * 64 *
          cdiv(T, T <= SHORT_STEPS * TILE_WAVES ? SHORT_STEPS : MIDDLE_STEPS);
 }

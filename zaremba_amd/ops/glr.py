@@ -24,7 +24,8 @@ tensors' device; on the CPU (or with ZAREMBA_AMD_FORCE_EAGER=1) it runs the
 eager math of ops/functional.py. All of them may be captured in a HIP graph;
 a captured training step calls glr_forward and glr_backward themselves, which
 need no autograd. Windows of up to 128 steps are one launch; longer ones two,
-with a workspace of 8 bytes for each channel and 128 steps (64 backward).
+with a workspace of 8 bytes for each channel and 128 steps (64 backward, and
+forward from 16384 channels on).
 """
 
 from __future__ import annotations
