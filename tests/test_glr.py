@@ -579,8 +579,9 @@ def test_refusals_of_shared_memory_and_sizes():
     in_h = h.view(-1)[5:5 + B * H].view(B, H)
     lengths = room[4:4 + B].view(torch.int32)
     grad = torch.zeros(T, B, H, device="cuda", requires_grad=True)
-    # 2^31 channels of one step would do, but not in 9: no such tensor is made
-    wide = torch.empty(1, 1, 4 * 32767, device="cuda").expand(9, 65536, -1)
+    # 2^31 channels of one step would do, but not of 17, which are 3 waves of
+    # 64 for each 64 channels: no such tensor is made
+    wide = torch.empty(1, 1, 4 * 32767, device="cuda").expand(17, 65536, -1)
     for call in (
             lambda: G.glr_forward(gates, in_h, out=h),
             lambda: G.glr_forward(gates, c0, lengths, out=h),

@@ -183,7 +183,11 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 // From SHARED_FROM groups of 64 channels on each of the 8 XCDs has a counter
 // and a share of the groups, neighbours side by side: rows of 64 values are
 // seldom whole cache lines, and the other halves are then met in the same L2.
-// With fewer groups each has a counter of its own, as the blocks of one would
+// (Blocks go round the XCDs in turn; no result depends on it.) Windows of one
+// tile have the same shares: in us, against groups in the blocks' order, 35 x
+// 20 x 1500 bf16 6.6 / 7.3 against 6.6 / 9.3 forward / backward, 100 x 20 x 1500
+// 9.3 / 17.4 against 12.0 / 21.5, 35 x 128 x 1500 17 / 33 against 22 / 45, rows of
+// whole lines (64 x 64 x 1024) the same. In a chain with fewer groups each has a counter of its own, as the blocks of one would
 // queue at one address (14 ns a slot) and an XCD would have 3 groups or less.
 // Measured in us, forward / backward in tiles of 8 waves, bf16, H = 1500: with
 // a counter a group against shares, 23.4 groups x 65536 steps 250 / 537 against
@@ -215,6 +219,22 @@ struct Slot {
   int order, group;
 };
 
+// The groups of XCD x.
+struct Share {
+  int first, count;
+
+  DEV_INLINE Share(const GlrArgs& a, int x)
+      : first(a.groups * x / XCDS),
+        count(a.groups * (x + 1) / XCDS - first) {}
+};
+
+// Of a window of one tile. The grid fits the largest share.
+DEV_INLINE Slot one_tile(const GlrArgs& a) {
+  const Share s(a, blockIdx.x % XCDS);
+  const int k = blockIdx.x / XCDS;
+  return {k < s.count ? 0 : 1, s.first + k};
+}
+
 struct Chain {
   uint64_t* words;  // [chunks, B * H]: A above C
   int64_t BH;
@@ -231,11 +251,11 @@ struct Chain {
       *lds = (int)__hip_atomic_fetch_add(
           reinterpret_cast<unsigned*>(a.work + x * COUNTER_APART), 1u,
           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const int first = shared ? a.groups * x / XCDS : x;
-    const int n = shared ? a.groups * (x + 1) / XCDS - first : 1;
+    const Share share(a, shared ? x : 0);
     __syncthreads();
     const int k = __builtin_amdgcn_readfirstlane(*lds);
-    return {min(k / n, a.chunks), first + k % n};
+    if (!shared) return {min(k, a.chunks), x};
+    return {min(k / share.count, a.chunks), share.first + k % share.count};
   }
 
   DEV_INLINE void publish(int slot, const Channel& ch, float A,
@@ -326,8 +346,8 @@ __global__ __launch_bounds__(64 * W) void glr_fwd_kernel(GlrArgs a) {
   const int waves = CHAIN ? W : blockDim.x / 64, lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
   const Slot slot =
-      CHAIN ? Chain::take_slot(a, &taken) : Slot{0, (int)blockIdx.x};
-  if (CHAIN && slot.order >= a.chunks) return;
+      CHAIN ? Chain::take_slot(a, &taken) : one_tile(a);
+  if (slot.order >= (CHAIN ? a.chunks : 1)) return;
   const Channel ch(a, slot.group);
   const E* g0 = static_cast<const E*>(a.gates) + ch.first * a.gates_b;
   E* h0 = static_cast<E*>(a.h) + ch.first * a.h_b;
@@ -399,8 +419,8 @@ __global__ __launch_bounds__(64 * W) void glr_bwd_kernel(GlrArgs a) {
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
   const int rw = waves - 1 - w;
   const Slot slot =
-      CHAIN ? Chain::take_slot(a, &taken) : Slot{0, (int)blockIdx.x};
-  if (CHAIN && slot.order >= a.chunks) return;
+      CHAIN ? Chain::take_slot(a, &taken) : one_tile(a);
+  if (slot.order >= (CHAIN ? a.chunks : 1)) return;
   const Channel ch(a, slot.group);
   const E* g0 = static_cast<const E*>(a.gates) + ch.first * a.gates_b;
   const E* dh0 = static_cast<const E*>(a.dh) + ch.first * a.dh_b;
@@ -529,22 +549,27 @@ void by_type(GlrType type, F f) {
   }
 }
 
-// Steps of a wave, and waves of a block. Up to 64 steps are a tile of waves
-// with 4 steps each (more waves to hide the one round of loads: 35 x 20 x 1500
-// bf16 takes 6.3 us against 6.8 with 8 each, 8.6 against 9.4 backward), up to
-// 128 one of waves with 8. A chain's tiles are 128 steps forward, 64 backward,
-// of 8 waves. 16 waves with 8 steps measured 218 us against 200 forward at
-// 65536 x 1 x 1472, 4 waves with 16 566 against 545 backward at 65536 x 1 x
-// 1500. Forward with MANY_GROUPS, a group for each CU, tiles are 64 steps of 4
-// waves: blocks end sooner, and more of them wait while others load. 300 x 64 x
-// 650 takes 34 us against 39, 512 x 80 x 1500 135 against 147 and with random
-// lengths 110 against 127, 1024 x 16 x 1500 56 against 60, but 256 x 20 x 1500
-// 21.8 against 21.3; with fewer groups 65536 x 1 x 1500 273 against 256, 8192 x 2
-// x 1024 f32 73 against 70. Backward the same costs 3 to 15 %. Blocks that loop over tiles, which need no chain, measured the same up to 128 steps, and from 256 steps
-// on up to four times a chain's time where channels are few (23 groups, 512
-// steps: 20 / 33 us against 10 / 14) and 1.1 to 1.4 times where they are many
-// (1875 groups, 512 steps: 161 / 401 against 153 / 292).
-constexpr int SHORT_STEPS = 4, MIDDLE_STEPS = 8, TILE_WAVES = 16;
+// Steps of a wave, and waves of a block. Up to 128 steps are one tile of waves
+// with 8 steps each, backward up to 64 of waves with 4: more waves to hide the
+// one round of loads. 35 x 20 x 1500 bf16 takes 7.3 us with 4 against 8.3, 16 x
+// 64 x 1500 8.1 against 9.5, but 64 x 128 x 650 23 against 21; forward 4 measure
+// 6.6 against 6.4, 17 against 16 at 35 x 128 x 1500, 14.5 against 12.6 at 64 x 128
+// x 650. From 65 steps on a chain would take 13 / 18 us at 65 x 20 x 1500 against
+// 7.2 / 11.4, and 58 / 116 against 57 / 125 at 128 x 128 x 1500.
+//
+// A chain's tiles are 128 steps forward, 64 backward, of 8 waves. 16 waves with
+// 8 steps measured 218 us against 200 forward at 65536 x 1 x 1472, 4 waves with
+// 16 566 against 545 backward at 65536 x 1 x 1500. Forward with MANY_GROUPS, a
+// group for each CU, tiles are 64 steps of 4 waves: blocks end sooner, and more
+// of them wait while others load. 300 x 64 x 650 takes 34 us against 39, 512 x 80
+// x 1500 135 against 147 and with random lengths 110 against 127, 1024 x 16 x 1500
+// 56 against 60, but 256 x 20 x 1500 21.8 against 21.3; with fewer groups 65536 x
+// 1 x 1500 273 against 256, 8192 x 2 x 1024 f32 73 against 70. Backward the same
+// costs 3 to 15 %. Blocks that loop over tiles, which need no chain, measured
+// from 256 steps on up to four times a chain's time where channels are few (23
+// groups, 512 steps: 20 / 33 us against 10 / 14) and 1.1 to 1.4 times where they
+// are many (1875 groups, 512 steps: 161 / 401 against 153 / 292).
+constexpr int TILE_STEPS = 8, SHORT_STEPS = 4, TILE_WAVES = 16;
 constexpr int FWD_STEPS = 16, BWD_STEPS = 8, CHAIN_WAVES = 8;
 constexpr int MANY_GROUPS = 256, MANY_WAVES = 4;
 
@@ -564,7 +589,7 @@ int chain_waves(int64_t groups, bool back) {
 
 // Tiles of a chain; 0 where one tile is the window.
 int chunks_of(int64_t T, int64_t groups, bool back) {
-  return T > MIDDLE_STEPS * TILE_WAVES
+  return T > TILE_STEPS * TILE_WAVES
              ? cdiv(T, (back ? BWD_STEPS : FWD_STEPS) *
                            chain_waves(groups, back))
              : 0;
@@ -577,15 +602,24 @@ GlrArgs planned(GlrArgs a, bool back, int size) {
   return a;
 }
 
-// At least as many for each counter as it has slots.
-int64_t chain_blocks(int64_t groups, int64_t chunks) {
-  return groups >= SHARED_FROM ? (int64_t)XCDS * cdiv(groups, XCDS) * chunks
-                               : (int64_t)XCDS * cdiv(chunks, XCDS) * groups;
+// Steps of a wave where one tile is the window.
+int tile_steps(int64_t T, bool back) {
+  return back && T <= SHORT_STEPS * TILE_WAVES ? SHORT_STEPS : TILE_STEPS;
+}
+
+// At least as many for each counter as it has slots, for each share as it has
+// groups.
+int64_t blocks_of(int64_t groups, int64_t chunks) {
+  return chunks && groups < SHARED_FROM
+             ? (int64_t)XCDS * cdiv(chunks, XCDS) * groups
+             : (int64_t)XCDS * cdiv(groups, XCDS) *
+                   std::max<int64_t>(chunks, 1);
 }
 
 template <bool BACK, typename E>
 void launch(const GlrArgs& args, hipStream_t stream) {
   GlrArgs a = planned(args, BACK, sizeof(E));
+  const int64_t blocks = blocks_of(a.groups, a.chunks);
   for (a.row0 = 0; a.row0 < a.B; a.row0 += a.rows) {
     if (a.chunks) {
       const int64_t n = glr_work_words(args, BACK, sizeof(E)) / 2;
@@ -596,18 +630,17 @@ void launch(const GlrArgs& args, hipStream_t stream) {
                     : waves == CHAIN_WAVES
                         ? glr_fwd_kernel<E, FWD_STEPS, CHAIN_WAVES, true>
                         : glr_fwd_kernel<E, FWD_STEPS, MANY_WAVES, true>;
-      hipLaunchKernelGGL(kernel, dim3(chain_blocks(a.groups, a.chunks)),
+      hipLaunchKernelGGL(kernel, dim3(blocks),
                          dim3(64 * waves), 0, stream, a);
-    } else if (a.T <= SHORT_STEPS * TILE_WAVES) {
-      auto kernel = BACK ? glr_bwd_kernel<E, SHORT_STEPS, TILE_WAVES, false>
-                         : glr_fwd_kernel<E, SHORT_STEPS, TILE_WAVES, false>;
-      hipLaunchKernelGGL(kernel, dim3(a.groups),
-                         dim3(64 * cdiv(a.T, SHORT_STEPS)), 0, stream, a);
     } else {
-      auto kernel = BACK ? glr_bwd_kernel<E, MIDDLE_STEPS, TILE_WAVES, false>
-                         : glr_fwd_kernel<E, MIDDLE_STEPS, TILE_WAVES, false>;
-      hipLaunchKernelGGL(kernel, dim3(a.groups),
-                         dim3(64 * cdiv(a.T, MIDDLE_STEPS)), 0, stream, a);
+      const int steps = tile_steps(a.T, BACK);
+      auto kernel = glr_fwd_kernel<E, TILE_STEPS, TILE_WAVES, false>;
+      if constexpr (BACK)
+        kernel = steps == TILE_STEPS
+                     ? glr_bwd_kernel<E, TILE_STEPS, TILE_WAVES, false>
+                     : glr_bwd_kernel<E, SHORT_STEPS, TILE_WAVES, false>;
+      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * cdiv(a.T, steps)), 0,
+                         stream, a);
     }
   }
 }
@@ -623,10 +656,8 @@ int64_t glr_work_words(const GlrArgs& args, bool back, int size) {
 
 int64_t glr_threads(int64_t T, int64_t B, int64_t H, bool back) {
   const int64_t groups = cdiv(B * H, 64), chunks = chunks_of(T, groups, back);
-  if (chunks)
-    return chain_blocks(groups, chunks) * 64 * chain_waves(groups, back);
-  return groups * 64 *
-         cdiv(T, T <= SHORT_STEPS * TILE_WAVES ? SHORT_STEPS : MIDDLE_STEPS);
+  return blocks_of(groups, chunks) * 64 *
+         (chunks ? chain_waves(groups, back) : cdiv(T, tile_steps(T, back)));
 }
 
 void launch_glr_fwd(const GlrArgs& a, GlrType type, hipStream_t stream) {
