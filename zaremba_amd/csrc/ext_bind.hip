@@ -15,6 +15,7 @@
 
 #include <array>
 #include <cstdint>
+#include <cstdlib>
 #include <map>
 #include <stdexcept>
 #include <vector>
@@ -614,7 +615,21 @@ static void transpose_bf16(const torch::Tensor& src, torch::Tensor& dst) {
 
 }  // namespace zamd
 
+namespace {
+
+PyObject* force_eager_env(PyObject*, PyObject*) {
+  const char* e = std::getenv("ZAREMBA_AMD_FORCE_EAGER");
+  return PyBool_FromLong(e != nullptr && e[0] == '1' && e[1] == 0);
+}
+
+PyMethodDef PLAIN[] = {
+    {"force_eager_env", force_eager_env, METH_NOARGS, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+
+}  // namespace
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  PyModule_AddFunctions(m.ptr(), PLAIN);  // no argument to convert
   m.doc() = "zaremba_amd gfx950 kernel library";
   m.def("gemm", &zamd::gemm, "MFMA bf16 GEMM (NT / TN)", py::arg("A"),
         py::arg("B"), py::arg("C"), py::arg("bias"), py::arg("trans_a"),
