@@ -370,3 +370,23 @@ def test_training_loop_runs(tmp_path, bits, capsys):
     assert int(opt2.step_count) == 2 * len(sets[0])
     for a, b in zip(opt.exp_avgs, opt2.exp_avgs):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@GPU
+@pytest.mark.parametrize("T", [1, 9, 200])
+@pytest.mark.parametrize("grad", [False, True])
+def test_hip_states_stay_as_returned(T, grad):
+    """The states of a window are not those of the window after it."""
+    m = model("hip", vocab=60, hidden=40).cuda()
+    with torch.set_grad_enabled(grad):
+        first, kept = None, None
+        for seed in (1, 2):
+            x, _ = batch(T, 3, 60, seed=seed, device="cuda")
+            _, states = m(x, m.state_init(3))
+            if first is None:
+                first = [(h, c) for h, c in states]
+                kept = [(h.clone(), c.clone()) for h, c in states]
+    for (h, c), (h0, c0), (h1, c1) in zip(first, kept, states):
+        assert torch.equal(h, h0) and torch.equal(c, c0)
+        assert not torch.equal(h, h1) and not torch.equal(c, c1)
+        assert not h.requires_grad and not c.requires_grad

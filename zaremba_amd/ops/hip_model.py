@@ -154,7 +154,6 @@ class _GlrWorkspace:
         bf = torch.bfloat16
         self.T, self.B, self.H = T, B, H
         self.gates = torch.zeros(T, B, 4 * H, dtype=bf, device=device)
-        self.h = torch.zeros(T, B, H, dtype=bf, device=device)
         # the dx GEMM's A operand, which over-reads into the slack
         self.dG = _slacked((T, B, 4 * H), bf, device, slack_ptrs)
         self.TBp = _pad64(T * B)
@@ -389,8 +388,9 @@ class HipModel:
 
     def _glr_layer(self, x, c0, layer, rt):
         if x.size(0) > 1 or torch.is_grad_enabled():
-            return GlrLayerFn.apply(x, c0, layer.W_x, layer.b_x, rt,
-                                    torch.is_grad_enabled())
+            out, c = GlrLayerFn.apply(x, c0, layer.W_x, layer.b_x, rt,
+                                      torch.is_grad_enabled())
+            return out, out.detach()[-1], c
         # one token: the state is advanced in place, in a copy of the
         # caller's
         B, H = x.size(1), rt.H

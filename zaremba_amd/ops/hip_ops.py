@@ -315,7 +315,7 @@ class GlrLayerFn(torch.autograd.Function):
     """One layer of the gated linear recurrence: the gate GEMM of the whole
     window, then the scan; backward the scan's gradient, then the batched
     dW / dx GEMMs as in LstmLayerFn. Workspaces are the layer runtime's (see
-    the aliasing contract above)."""
+    the aliasing contract above); what is returned is the call's own."""
 
     @staticmethod
     def forward(ctx, x, c0, Wx_m, bx_m, rt, training):
@@ -326,15 +326,14 @@ class GlrLayerFn(torch.autograd.Function):
         e.gemm(x2.view(T * B, Hin), rt.Wx, ws.gates.view(T * B, 4 * rt.H),
                bx_m, False, False)
         c0 = c0.to(torch.float32)
-        _, cT, marks = e.glr_forward(ws.gates, c0, None, training, ws.h)
-        out, hT = ws.h[:], ws.h[T - 1]  # views: ws.h itself joins no graph
+        out, cT, marks = e.glr_forward(ws.gates, c0, None, training, None)
         ctx.save_for_backward(x2, c0, marks)
         ctx.rt = rt
-        ctx.mark_non_differentiable(hT, cT)
-        return out, hT, cT
+        ctx.mark_non_differentiable(cT)
+        return out, cT
 
     @staticmethod
-    def backward(ctx, dY, dhT, dcT):
+    def backward(ctx, dY, dcT):
         x2, c0, marks = ctx.saved_tensors
         rt = ctx.rt
         ws = rt.ws
