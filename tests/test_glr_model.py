@@ -390,3 +390,53 @@ def test_hip_states_stay_as_returned(T, grad):
         assert torch.equal(h, h0) and torch.equal(c, c0)
         assert not torch.equal(h, h1) and not torch.equal(c, c1)
         assert not h.requires_grad and not c.requires_grad
+
+
+@GPU
+@pytest.mark.parametrize("layers", [1, 2])
+@pytest.mark.parametrize("dropout", [0.0, 0.5])
+@pytest.mark.parametrize("between", [(9, 4, True), (9, 4, False),
+                                     (4, 9, True), (3, 4, False)])
+def test_hip_backward_of_an_older_window_is_refused(layers, dropout, between):
+    """Its workspaces hold what came between; the newest window's gradients
+    are those that it has by itself."""
+    T, B, train = between
+    m = model("hip", vocab=60, hidden=40, layers=layers,
+              dropout=dropout).cuda()
+
+    def window(seed, T, B):
+        x, y = batch(T, B, 60, seed=seed, device="cuda")
+        scores, _ = m(x, m.state_init(B))
+        return trainer.nll_loss(scores, y)
+
+    old = window(1, 9, 4)
+    m.train(train)
+    with torch.set_grad_enabled(train):
+        new = window(2, T, B)
+    with pytest.raises(RuntimeError, match="another forward pass"):
+        old.backward()
+    if not train:
+        return
+    m.zero_grad()
+    new.backward()
+    got = [p.grad.clone() for p in m.parameters()]
+    if dropout:  # other masks
+        return
+    m.zero_grad()
+    window(2, T, B).backward()
+    # the embedding's gradients are added up in any order
+    for a, p in zip(got[1:], list(m.parameters())[1:]):
+        assert torch.equal(a, p.grad)
+
+
+@GPU
+def test_hip_token_after_a_window_of_one_step():
+    """One token without gradients overwrites a one-step window's gates."""
+    m = model("hip", vocab=60, hidden=40).cuda()
+    x, y = batch(1, 4, 60, device="cuda")
+    scores, _ = m(x, m.state_init(4))
+    loss = trainer.nll_loss(scores, y)
+    with torch.no_grad():
+        m(x, m.state_init(4))
+    with pytest.raises(RuntimeError, match="another forward pass"):
+        loss.backward()

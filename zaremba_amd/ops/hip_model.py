@@ -171,6 +171,7 @@ class _GlrRuntime:
         self.H4p = _pad64(4 * self.H)  # see _LayerRuntime
         self.WxT = torch.zeros(self.Hin, self.H4p, dtype=bf, device=device)
         self.ws: Optional[_GlrWorkspace] = None
+        self.passes = 0  # forward passes that have used the workspaces
         self.slack_ptrs = None
         self.dx_part = None
         self.xT_buf = None
@@ -394,6 +395,7 @@ class HipModel:
         # one token: the state is advanced in place, in a copy of the
         # caller's
         B, H = x.size(1), rt.H
+        rt.passes += 1
         gates = rt.ws.gates.view(B, 4 * H)
         self.e.gemm(x.reshape(B, -1).contiguous(), rt.Wx, gates, layer.b_x,
                     False, False)

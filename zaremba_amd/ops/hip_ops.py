@@ -315,7 +315,8 @@ class GlrLayerFn(torch.autograd.Function):
     """One layer of the gated linear recurrence: the gate GEMM of the whole
     window, then the scan; backward the scan's gradient, then the batched
     dW / dx GEMMs as in LstmLayerFn. Workspaces are the layer runtime's (see
-    the aliasing contract above); what is returned is the call's own."""
+    the aliasing contract above), and a backward pass that comes too late for
+    them is refused; what is returned is the call's own."""
 
     @staticmethod
     def forward(ctx, x, c0, Wx_m, bx_m, rt, training):
@@ -323,12 +324,13 @@ class GlrLayerFn(torch.autograd.Function):
         x2 = x.contiguous()
         e = ext()
         ws = rt.ws
+        rt.passes += 1
         e.gemm(x2.view(T * B, Hin), rt.Wx, ws.gates.view(T * B, 4 * rt.H),
                bx_m, False, False)
         c0 = c0.to(torch.float32)
         out, cT, marks = e.glr_forward(ws.gates, c0, None, training, None)
         ctx.save_for_backward(x2, c0, marks)
-        ctx.rt = rt
+        ctx.rt, ctx.passes = rt, rt.passes
         ctx.mark_non_differentiable(cT)
         return out, cT
 
@@ -336,6 +338,11 @@ class GlrLayerFn(torch.autograd.Function):
     def backward(ctx, dY, dcT):
         x2, c0, marks = ctx.saved_tensors
         rt = ctx.rt
+        if ctx.passes != rt.passes:
+            raise RuntimeError(
+                "GLR layer: another forward pass of this model came between "
+                "a forward pass and its backward pass, and has overwritten "
+                "the gates that this one needs")
         ws = rt.ws
         e = ext()
         T, B, Hin = x2.shape
