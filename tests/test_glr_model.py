@@ -440,3 +440,18 @@ def test_hip_token_after_a_window_of_one_step():
         m(x, m.state_init(4))
     with pytest.raises(RuntimeError, match="another forward pass"):
         loss.backward()
+
+
+@GPU
+def test_hip_layer_has_no_second_derivative():
+    m = model("hip", vocab=60, hidden=40, layers=1).cuda()
+    x, _ = batch(5, 3, 60, device="cuda")
+    m(x, m.state_init(3))
+    hm, layer = m._hip_model, m.rnns[0]
+    cur = torch.randn(5, 3, 40, device="cuda").bfloat16().requires_grad_()
+    out, _, _ = hm._glr_layer(cur, torch.zeros(3, 40, device="cuda"), layer,
+                              hm.layers[0])
+    (d,) = torch.autograd.grad(out.float().square().sum(), cur,
+                               create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable"):
+        d.float().sum().backward()

@@ -335,6 +335,7 @@ class GlrLayerFn(torch.autograd.Function):
         return out, cT
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dY, dcT):
         x2, c0, marks = ctx.saved_tensors
         rt = ctx.rt
