@@ -629,3 +629,26 @@ def test_windows_of_many_channels(T, B, H, dtype):
         assert torch.equal(again[0], h) and torch.equal(again[1], cT)
         back = G.glr_backward(dh, dcT, gates, c0, again[2], lengths)
         assert torch.equal(back[0], dgates) and torch.equal(back[1], dc0)
+
+
+@GPU
+def test_tangents_are_refused():
+    """The kernels would drop them."""
+    import torch.autograd.forward_ad as fwd
+    gates, c0, dh, dcT, _ = make(5, 3, 4, torch.float32, "cuda")
+    _, _, marks = G.glr_forward(gates, c0, training=True)
+    with fwd.dual_level():
+        dual = lambda x: fwd.make_dual(x, torch.ones_like(x))  # noqa: E731
+        g, c, d, e = (dual(x) for x in (gates, c0, dh, dcT))
+        for call in (
+                lambda: G.glr(g, c0), lambda: G.glr(gates, c),
+                lambda: G.glr(g.clone().requires_grad_(), c0),
+                lambda: G.glr_forward(g, c0), lambda: G.glr_forward(gates, c),
+                lambda: G.glr_backward(d, dcT, gates, c0, marks),
+                lambda: G.glr_backward(dh, e, gates, c0, marks),
+                lambda: G.glr_backward(dh, dcT, g, c0, marks),
+                lambda: G.glr_step(g[0], c0),
+                lambda: G.glr_step(gates[0], c.clone())):
+            with pytest.raises(RuntimeError, match="forward|jvp|tangent"):
+                call()
+        G.glr(gates, c0)  # others beside them are not

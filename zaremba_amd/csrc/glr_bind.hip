@@ -30,6 +30,12 @@ GlrType glr_type(const Tensor& t, const char* op) {
   }
 }
 
+// The kernels hand no tangent on.
+void check_no_tangent(const Tensor& x, const char* op, const char* name) {
+  TORCH_CHECK(!x._fw_grad(0).defined(), op, ": ", name, " has a tangent; "
+              "there is no forward-mode derivative");
+}
+
 void check_gates(const Tensor& gates, int64_t dims, const char* op,
                  bool back = false) {
   TORCH_CHECK(gates.is_cuda(), op, ": gates must be on the GPU");
@@ -38,6 +44,7 @@ void check_gates(const Tensor& gates, int64_t dims, const char* op,
   TORCH_CHECK(gates.size(-1) % 4 == 0, op,
               ": the last axis of gates holds the 4 gates, got ",
               gates.size(-1), " values");
+  check_no_tangent(gates, op, "gates");
   const int64_t B = gates.size(-2), H = gates.size(-1) / 4;
   TORCH_CHECK(B * H < std::numeric_limits<int>::max() - 64 &&
               (dims == 2 ||
@@ -56,6 +63,7 @@ Tensor state_like(const Tensor& c, const Tensor& gates, const char* op,
               c.device(), " and gates on ", gates.device());
   TORCH_CHECK(c.dim() == 2 && c.size(0) == B && c.size(1) == H, op, ": ",
               name, " must be [", B, ", ", H, "], got ", c.sizes());
+  check_no_tangent(c, op, name);
   return c.contiguous();
 }
 
@@ -226,6 +234,7 @@ std::tuple<Tensor, Tensor> glr_backward(
                 dh_in->size(1) == a.B && dh_in->size(2) == a.H,
                 op, ": dh must be [", a.T, ", ", a.B, ", ", a.H, "], got ",
                 dh_in->sizes());
+    check_no_tangent(*dh_in, op, "dh");
     dh = dense_rows(*dh_in);
   } else {
     dh = torch::zeros({1, 1, a.H}, gates.options()).expand({a.T, a.B, a.H});
@@ -287,6 +296,7 @@ Tensor glr_step(const Tensor& gates_in, const Tensor& c) {
               (a.B <= 1 || c.stride(0) >= a.H),
               op, ": the rows of c must be dense and apart, got strides ",
               c.strides());
+  check_no_tangent(c, op, "c");
   TORCH_CHECK(!overlap(c, gates), op, ": c shares memory with gates");
   Tensor h = torch::empty({a.B, a.H}, gates.options());
   if (h.numel() == 0) return h;

@@ -148,7 +148,8 @@ class GlrFn(torch.autograd.Function):
 
 
 def glr(gates, c0=None, lengths=None):
-    """``(h, cT)``, differentiable in ``gates`` and ``c0``."""
+    """``(h, cT)``, differentiable in ``gates`` and ``c0``: once, and on the
+    GPU in reverse mode only (a tensor with a tangent is refused)."""
     if not _eager(gates):
         if torch.is_grad_enabled() and (
                 gates.requires_grad or (c0 is not None and c0.requires_grad)):
