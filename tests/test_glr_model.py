@@ -455,3 +455,60 @@ def test_hip_layer_has_no_second_derivative():
                                create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable"):
         d.float().sum().backward()
+
+
+@GPU
+@pytest.mark.parametrize("T", [129, 400])
+def test_hip_a_wait_that_ends_is_told(T):
+    """No look at all is allowed: every tile but the first gives up. The
+    kernels end, states are NaN, and check_aborts raises."""
+    from zaremba_amd import _C
+    e = _C.ext()
+    x, y = batch(T, 3, 60, device="cuda")
+    m = model("hip", vocab=60, hidden=40).cuda()
+    scores, states = m(x, m.state_init(3))
+    trainer.nll_loss(scores, y).backward()
+    m._hip_model.check_aborts()
+    m = model("hip", vocab=60, hidden=40, layers=1).cuda()
+    e.set_glr_polls(0)
+    try:
+        with torch.no_grad():
+            short, _ = m(x[:128], m.state_init(3))
+            m._hip_model.check_aborts()      # one tile waits for nobody
+            scores, states = m(x, m.state_init(3))
+        torch.cuda.synchronize()
+    finally:
+        e.set_glr_polls(1 << 22)
+    assert bool(torch.isnan(states[0][1]).all())
+    scores = scores.view(T, 3, -1)
+    assert not torch.isnan(scores[:128]).any()
+    assert bool(torch.isnan(scores[128:]).all())
+    with pytest.raises(RuntimeError, match="gave up"):
+        m._hip_model.check_aborts()
+    # in the backward pass alone
+    m = model("hip", vocab=60, hidden=40, layers=1).cuda()
+    scores, _ = m(x, m.state_init(3))
+    m._hip_model.check_aborts()
+    e.set_glr_polls(0)
+    try:
+        trainer.nll_loss(scores, y).backward()
+        torch.cuda.synchronize()
+    finally:
+        e.set_glr_polls(1 << 22)
+    assert bool(torch.isnan(m.rnns[0].W_x.grad).any())
+    with pytest.raises(RuntimeError, match="gave up"):
+        m._hip_model.check_aborts()
+
+
+@GPU
+def test_gave_up_is_checked():
+    from zaremba_amd import _C
+    e = _C.ext()
+    gates = torch.zeros(4, 3, 8, device="cuda")
+    for bad in (torch.zeros(1, device="cuda"),
+                torch.zeros(2, dtype=torch.int32, device="cuda"),
+                torch.zeros(1, dtype=torch.int32)):
+        with pytest.raises(RuntimeError, match="gave_up"):
+            e.glr_forward(gates, None, None, False, None, bad)
+    with pytest.raises(RuntimeError, match="set_glr_polls"):
+        e.set_glr_polls(-1)

@@ -200,7 +200,8 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 // Blocks take their slots from counters as they start. A block therefore
 // waits only for blocks that run already, and these only for earlier ones:
 // every wait ends, whatever the number of blocks that fit the chip. Polls are
-// bounded all the same; behind a bound that is reached the state is NaN.
+// bounded all the same; behind a bound that is reached the state is NaN, and
+// a flag says so.
 //
 // From SHARED_FROM groups of 64 channels on each of the 8 XCDs has a counter
 // and a share of the groups, neighbours side by side: rows of 64 values are
@@ -225,7 +226,6 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 // in a launch of its own, which reads three gates twice, took 360 and 680, and
 // a block that loops over its tiles 2380 and 4500.
 constexpr unsigned ABSENT = 0xffffffffu;
-constexpr int MOST_POLLS = 1 << 22;
 constexpr int XCDS = 8;
 constexpr int SHARED_FROM = 32;    // groups: a counter for each XCD
 constexpr int COUNTER_APART = 16;  // words: 128 bytes
@@ -260,9 +260,12 @@ DEV_INLINE Slot one_tile(const GlrArgs& a) {
 struct Chain {
   uint64_t* words;  // [chunks, B * H]: A above C
   int64_t BH;
+  int most_polls;
+  unsigned* gave_up;
 
   DEV_INLINE Chain(const GlrArgs& a)
-      : words(a.work + COUNTER_WORDS), BH((int64_t)a.B * a.H) {}
+      : words(a.work + COUNTER_WORDS), BH((int64_t)a.B * a.H),
+        most_polls(a.polls), gave_up(a.gave_up) {}
 
   // A counter deals out the slots of its groups in order. It gets at least as
   // many blocks as slots: order a.chunks is none.
@@ -294,6 +297,13 @@ struct Chain {
     float c = start;
     int n = 0;  // slots before this one whose words are kept in `seen`
     for (int polls = 0; n < slot;) {
+      if (polls == most_polls) {
+        c = __builtin_nanf("");
+        if (gave_up && lane_id() == 0)
+          __hip_atomic_store(gave_up, 1u, __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
+        break;
+      }
       uint64_t p[DEPTH];
 #pragma unroll
       for (int q = 0; q < DEPTH; ++q)
@@ -318,10 +328,7 @@ struct Chain {
       }
       if (met) break;
       if (!more) {
-        if (++polls == MOST_POLLS) {
-          c = __builtin_nanf("");
-          break;
-        }
+        ++polls;
         __builtin_amdgcn_s_sleep(1);
       }
     }

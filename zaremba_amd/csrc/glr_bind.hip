@@ -139,6 +139,24 @@ void set_sizes(GlrArgs& a, const Tensor& gates) {
   a.gates_b = gates.stride(1);
 }
 
+int g_polls = GLR_POLLS;
+
+// For tests: how often a block looks for a state before it gives up.
+void set_glr_polls(int n) {
+  TORCH_CHECK(n >= 0, "set_glr_polls: must not be negative, got ", n);
+  g_polls = n;
+}
+
+void set_waits(GlrArgs& a, const OptTensor& gave_up, const Tensor& gates,
+               const char* op) {
+  a.polls = g_polls;
+  if (!gave_up) return;
+  TORCH_CHECK(gave_up->scalar_type() == torch::kInt32 &&
+              gave_up->numel() == 1 && gave_up->device() == gates.device(),
+              op, ": gave_up must be one int32 on the gates' device");
+  a.gave_up = reinterpret_cast<unsigned*>(gave_up->data_ptr<int>());
+}
+
 int64_t mark_count(int64_t T) { return (T + GLR_MARK - 1) / GLR_MARK; }
 
 // A workspace of this call alone: the caching allocator keeps those of other
@@ -153,7 +171,7 @@ Tensor workspace(GlrArgs& a, bool back, const Tensor& gates) {
 
 std::tuple<Tensor, Tensor, OptTensor> glr_forward(
     const Tensor& gates_in, const OptTensor& c0_in, const OptTensor& lengths,
-    bool training, const OptTensor& out) {
+    bool training, const OptTensor& out, const OptTensor& gave_up) {
   const char* op = "glr_forward";
   check_gates(gates_in, 3, op);
   const GlrType type = glr_type(gates_in, op);
@@ -161,6 +179,7 @@ std::tuple<Tensor, Tensor, OptTensor> glr_forward(
   const Tensor gates = dense_rows(gates_in);
   GlrArgs a;
   set_sizes(a, gates);
+  set_waits(a, gave_up, gates, op);
   Tensor keep, c0;
   set_lengths(a, lengths, keep, gates, op);
   if (c0_in) {
@@ -200,7 +219,7 @@ std::tuple<Tensor, Tensor, OptTensor> glr_forward(
 std::tuple<Tensor, Tensor> glr_backward(
     const OptTensor& dh_in, const OptTensor& dcT_in, const Tensor& gates_in,
     const OptTensor& c0_in, const Tensor& marks, const OptTensor& lengths,
-    const OptTensor& out) {
+    const OptTensor& out, const OptTensor& gave_up) {
   const char* op = "glr_backward";
   check_gates(gates_in, 3, op, true);
   const GlrType type = glr_type(gates_in, op);
@@ -208,6 +227,7 @@ std::tuple<Tensor, Tensor> glr_backward(
   const Tensor gates = dense_rows(gates_in);
   GlrArgs a;
   set_sizes(a, gates);
+  set_waits(a, gave_up, gates, op);
   Tensor keep, c0, dcT, dh;
   set_lengths(a, lengths, keep, gates, op);
   if (c0_in) {
@@ -316,10 +336,13 @@ Tensor glr_step(const Tensor& gates_in, const Tensor& c) {
 
 void bind_glr(py::module_& m) {
   m.def("glr_forward", &glr_forward, py::arg("gates"), py::arg("c0"),
-        py::arg("lengths"), py::arg("training"), py::arg("out"));
+        py::arg("lengths"), py::arg("training"), py::arg("out"),
+        py::arg("gave_up") = py::none());
   m.def("glr_backward", &glr_backward, py::arg("dh"), py::arg("dcT"),
         py::arg("gates"), py::arg("c0"), py::arg("marks"),
-        py::arg("lengths"), py::arg("out"));
+        py::arg("lengths"), py::arg("out"),
+        py::arg("gave_up") = py::none());
+  m.def("set_glr_polls", &set_glr_polls);
   m.def("glr_step", &glr_step, py::arg("gates"), py::arg("c"));
 }
 

@@ -78,6 +78,7 @@ void launch_lstm_persistent_bwd(const bf16* dY, const bf16* rec,
 // the state of launch_glr_step (cT, read and written), whose rows are c_b
 // apart.
 constexpr int GLR_MARK = 32;  // steps between two kept states
+constexpr int GLR_POLLS = 1 << 22;  // looks at a state that is not there yet
 enum class GlrType { F32, F16, BF16 };
 struct GlrArgs {
   const void* gates = nullptr;  // [T, B, 4H]
@@ -101,6 +102,11 @@ struct GlrArgs {
   // set by the launchers: the rows of a launch, its blocks of 64 channels
   // and chunks of time
   int row0 = 0, rows = 0, groups = 0, chunks = 0;
+  // A block whose state has not come after so many looks goes on with NaN and
+  // sets *gave_up to 1, unless that is null. (Last: ahead of the sizes they
+  // cost a short window 0.2 us, as the sizes then lie in another line.)
+  int polls = GLR_POLLS;
+  unsigned* gave_up = nullptr;
 };
 // Words of 64 bits that a call needs for itself; size: of a gate in bytes.
 int64_t glr_work_words(const GlrArgs& a, bool back, int size);

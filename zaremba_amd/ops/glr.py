@@ -25,7 +25,8 @@ eager math of ops/functional.py. All of them may be captured in a HIP graph;
 a captured training step calls glr_forward and glr_backward themselves, which
 need no autograd. Windows of up to 128 steps are one launch; longer ones two,
 with a workspace of 8 bytes for each channel and 128 steps (64 backward, and
-forward from 16384 channels on).
+forward from 16384 channels on). Their blocks wait for each other, a bounded
+time: should one ever give up, the states from its steps on are NaN.
 """
 
 from __future__ import annotations

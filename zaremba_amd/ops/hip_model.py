@@ -125,6 +125,9 @@ class _LayerRuntime:
         self.xT_buf = None   # persistent [Hin, TBp] transposed-x temp
         self.owner = None    # back-ref to the HipModel (side stream)
 
+    def aborted(self):
+        return self.ws is not None and int(self.ws.abort.item()) != 0
+
     def shadows(self, layer):
         return [(layer.W_x, self.Wx), (layer.W_h, self.Wh)]
 
@@ -172,10 +175,14 @@ class _GlrRuntime:
         self.WxT = torch.zeros(self.Hin, self.H4p, dtype=bf, device=device)
         self.ws: Optional[_GlrWorkspace] = None
         self.passes = 0  # forward passes that have used the workspaces
+        self.abort = torch.zeros(1, dtype=torch.int32, device=device)
         self.slack_ptrs = None
         self.dx_part = None
         self.xT_buf = None
         self.owner = None
+
+    def aborted(self):
+        return int(self.abort.item()) != 0
 
     def shadows(self, layer):
         return [(layer.W_x, self.Wx)]
@@ -311,15 +318,18 @@ class HipModel:
         self._shadows_fresh = False
 
     def check_aborts(self):
-        """Raise if any grid-synchronized kernel hit its bounded-spin
-        timeout (the abort flag makes blocks EXIT instead of hanging the
-        GPU, but the step's outputs are then garbage). Called from the
-        trainer's log steps, which synchronize anyway — failure detection
-        at zero steady-state cost."""
-        if self.model.cell != "lstm":
-            return  # no such kernels
+        """Raise if any kernel whose blocks wait for each other hit its
+        bounded-spin timeout (the abort flag makes blocks EXIT instead of
+        hanging the GPU, but the step's outputs are then garbage). Called
+        from the trainer's log steps, which synchronize anyway — failure
+        detection at zero steady-state cost."""
         for rt in self.layers:
-            if rt.ws is not None and int(rt.ws.abort.item()) != 0:
+            if rt.aborted() and self.model.cell == "glr":
+                raise RuntimeError(
+                    "linear recurrence aborted (bounded-spin timeout): a "
+                    "block gave up waiting for the state before its steps; "
+                    "the affected step's states are NaN.")
+            if rt.aborted():
                 raise RuntimeError(
                     "persistent/fused LSTM kernel aborted (bounded-spin "
                     "timeout): a co-residency or synchronization failure; "

@@ -328,7 +328,8 @@ class GlrLayerFn(torch.autograd.Function):
         e.gemm(x2.view(T * B, Hin), rt.Wx, ws.gates.view(T * B, 4 * rt.H),
                bx_m, False, False)
         c0 = c0.to(torch.float32)
-        out, cT, marks = e.glr_forward(ws.gates, c0, None, training, None)
+        out, cT, marks = e.glr_forward(ws.gates, c0, None, training, None,
+                                       rt.abort)
         ctx.save_for_backward(x2, c0, marks)
         ctx.rt, ctx.passes = rt, rt.passes
         ctx.mark_non_differentiable(cT)
@@ -349,7 +350,7 @@ class GlrLayerFn(torch.autograd.Function):
         T, B, Hin = x2.shape
         TB, H = T * B, rt.H
         e.glr_backward(dY.to(torch.bfloat16), None, ws.gates, c0, marks,
-                       None, ws.dG)
+                       None, ws.dG, rt.abort)
         dG2 = ws.dG.view(TB, 4 * H)
         # dW_x = dG^T @ x over transposed, zero-padded temps (LstmLayerFn)
         e.transpose_bf16(dG2, ws.dGT)
