@@ -93,7 +93,7 @@ struct GlrArgs {
   float* cT = nullptr;
   int64_t c_b = 0;
   const float* dcT = nullptr;   // null: zeros
-  float* dc0 = nullptr;         // null: not wanted
+  float* dc0 = nullptr;         // not null
   float* marks = nullptr;       // [ceil(T / GLR_MARK), B, H]; null: not kept
   const void* lengths = nullptr;  // [B] int32 or int64; null: all T
   bool lengths_64 = false;
