@@ -29,7 +29,8 @@ from zaremba_amd.ensemble_eval import (ensemble_perplexity,
 from zaremba_amd.models.lstm_lm import Model
 from zaremba_amd.parallel import dist as zdist
 
-from main import make_optimizer, setdevice  # same policies/messages
+from main import (make_optimizer, set_learning_rate,  # same policies
+                  setdevice)
 
 
 def build_parser():
@@ -54,8 +55,9 @@ def build_parser():
                         help="The batch size.")
     parser.add_argument("--seq_length", type=int, default=20,
                         help="The sequence length for bptt.")
-    parser.add_argument("--learning_rate", type=float, default=1,
-                        help="The learning rate.")
+    parser.add_argument("--learning_rate", type=float, default=None,
+                        help="The learning rate. Default 1, as in the "
+                             "reference; 0.001 under AdamW.")
     parser.add_argument("--total_epochs", type=int, default=13,
                         help="Total number of epochs for training.")
     parser.add_argument("--factor_epoch", type=int, default=4,
@@ -137,6 +139,7 @@ def jsonl_for_model(args, model_num):
 
 def main():
     args = build_parser().parse_args()
+    set_learning_rate(args)
     if args.engine == "hip" and args.dtype == "fp32":
         raise SystemExit(
             "--dtype fp32 is not supported by --engine hip (bf16 compute / "

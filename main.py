@@ -42,8 +42,9 @@ def build_parser():
                         help="The batch size (per GPU under data parallelism).")
     parser.add_argument("--seq_length", type=int, default=35,
                         help="The sequence length for bptt.")
-    parser.add_argument("--learning_rate", type=float, default=1,
-                        help="The learning rate.")
+    parser.add_argument("--learning_rate", type=float, default=None,
+                        help="The learning rate. Default 1, as in the "
+                             "reference; 0.001 under AdamW.")
     parser.add_argument("--total_epochs", type=int, default=39,
                         help="Total number of epochs for training.")
     parser.add_argument("--factor_epoch", type=int, default=6,
@@ -128,6 +129,13 @@ def load_data(args):
     return zdata.data_init(args.data_dir)
 
 
+def set_learning_rate(args):
+    """The optimizer's default where none was given. AdamW moves a weight by
+    about the rate at each step, whatever the size of its gradient."""
+    if args.learning_rate is None:
+        args.learning_rate = 1 if args.optimizer == "sgd" else 1e-3
+
+
 def make_optimizer(args, model):
     """None for the reference's SGD, which the trainer does itself."""
     if args.optimizer == "sgd":
@@ -139,6 +147,7 @@ def make_optimizer(args, model):
 
 def main():
     args = build_parser().parse_args()
+    set_learning_rate(args)
     if args.engine == "hip" and args.dtype == "fp32":
         # The HIP kernel path is bf16-compute / fp32-master by design;
         # refuse up front rather than silently computing in bf16.

@@ -123,3 +123,26 @@ def test_ensemble_jsonl_per_model_suffix(monkeypatch):
     assert ens.jsonl_for_model(A, 3) == "/tmp/run.model3.jsonl"
     A.jsonl = None
     assert ens.jsonl_for_model(A, 1) is None
+
+
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("optimizer,rate", [("sgd", 1.0), ("adamw", 1e-3),
+                                            ("adamw8bit", 1e-3)])
+@pytest.mark.parametrize("script", ["main.py", "ensemble.py"])
+def test_default_rate_is_the_optimizers(tmp_path, script, optimizer, rate):
+    """SGD's rate of 1 would move every weight by 1 a step under AdamW."""
+    jl = str(tmp_path / "log.jsonl")
+    args = [script, "--device", "cpu", "--data",
+            "synthetic:vocab=40,tokens=1500", "--hidden_size", "8",
+            "--layer_num", "1", "--seq_length", "8", "--batch_size", "4",
+            "--total_epochs", "1", "--optimizer", optimizer]
+    if script == "ensemble.py":
+        args += ["--ensemble_num", "1"]
+    r = run_cli(args + ["--jsonl", jl])
+    assert r.returncode == 0, r.stderr[-2000:]
+    rates = {e["lr"] for e in map(json.loads, open(jl)) if "lr" in e}
+    assert rates == {rate}
+    r = run_cli(args + ["--jsonl", jl + "2", "--learning_rate", "0.25"])
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert {e["lr"] for e in map(json.loads, open(jl + "2"))
+            if "lr" in e} == {0.25}
