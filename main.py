@@ -206,6 +206,9 @@ def main():
         dp = GradBucketer(model)
 
     optimizer = make_optimizer(args, model)
+    if resumed is not None and optimizer is None and "optimizer" in resumed:
+        raise SystemExit(f"{args.resume} was saved under AdamW: pass the "
+                         "--optimizer that it was trained with")
     if resumed is not None and optimizer is not None:
         if "optimizer" not in resumed:
             raise SystemExit(f"{args.resume} holds no optimizer states: it "

@@ -152,6 +152,20 @@ def test_cli_refuses_states_that_were_not_saved(tmp_path):
 
 
 @pytest.mark.timeout(300)
+def test_cli_does_not_drop_states(tmp_path):
+    """An AdamW run that is resumed without naming AdamW."""
+    ck = str(tmp_path / "m.pt")
+    args = ["main.py", "--device", "cpu", "--data",
+            "synthetic:vocab=40,tokens=1500", "--hidden_size", "8",
+            "--layer_num", "1", "--seq_length", "8", "--batch_size", "4"]
+    r = run_cli(args + ["--total_epochs", "1", "--optimizer", "adamw",
+                        "--save", ck])
+    assert r.returncode == 0, r.stderr[-2000:]
+    r = run_cli(args + ["--total_epochs", "2", "--resume", ck])
+    assert r.returncode != 0 and "saved under AdamW" in r.stderr
+
+
+@pytest.mark.timeout(300)
 def test_ensemble_cli(tmp_path):
     r = run_cli(["ensemble.py", "--device", "cpu", "--data",
                  "synthetic:vocab=40,tokens=3000", "--hidden_size", "16",
