@@ -277,6 +277,28 @@ def test_state_dict_round_trip(bits):
     assert torch.equal(p[1], keep)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_saved_state_stays_as_it_was(bits):
+    """Going back to it after more steps gives the same steps again."""
+    torch.manual_seed(0)
+    p = torch.nn.Parameter(torch.randn(300))
+    opt = A.AdamW([p], bits=bits)
+
+    def steps():
+        gen = torch.Generator().manual_seed(3)
+        for _ in range(3):
+            p.grad = torch.randn(300, generator=gen)
+            opt.step(0.01, 1.0)
+        return p.detach().clone()
+
+    steps()
+    saved, start = opt.state_dict(), p.detach().clone()
+    first = steps()
+    opt.load_state_dict(saved)
+    p.data.copy_(start)
+    assert torch.equal(steps(), first)
+
+
 # ---------------------------------------------------------------------------
 # kernels
 # ---------------------------------------------------------------------------

@@ -140,10 +140,12 @@ class AdamW:
               "exp_avg_sq_scales")
 
     def state_dict(self):
-        out = {"bits": self.bits, "step_count": self.step_count.cpu()}
+        """A copy on the CPU, which later steps leave as it is."""
+        copy = lambda t: t.to("cpu", copy=True)  # noqa: E731
+        out = {"bits": self.bits, "step_count": copy(self.step_count)}
         for name in self._LISTS:
             x = getattr(self, name)
-            out[name] = None if x is None else [t.cpu() for t in x]
+            out[name] = None if x is None else [copy(t) for t in x]
         return out
 
     def load_state_dict(self, state):
