@@ -19,3 +19,10 @@ def pytest_collection_modifyitems(config, items):
     for item in items:
         if "gpu" in item.keywords:
             item.add_marker(skip_gpu)
+
+
+@pytest.fixture(autouse=True)
+def same_numbers_every_run():
+    """A test that draws without a seed of its own draws the same each time:
+    torch seeds itself anew in every process."""
+    torch.manual_seed(0)

@@ -173,6 +173,29 @@ def test_draw_is_right_in_the_mean():
     assert int((codes.amax(1) - codes.amin(1)).max()) == 1
 
 
+@pytest.mark.parametrize("seed", [0, 2, 10, 45, 62, 165])
+def test_draw_is_right_between_its_neighbours(seed):
+    """The same at values that lie so near a code that 4096 even draws may
+    all give it, and anywhere else: off by one draw of the gap between the
+    neighbours, not of the codes that were drawn."""
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.cat([torch.rand(300, generator=gen) * 448,
+                   torch.rand(200, generator=gen) * 2.0 ** -5 + 2.0 ** -9])
+    value = torch.arange(127, dtype=torch.uint8).view(E4M3).float()
+    near = value[2:126, None] * (1 + torch.tensor([[-1e-5, -1e-6, 0, 1e-6,
+                                                    1e-5]]))
+    x = torch.cat([x, near.flatten()])
+    low = torch.searchsorted(value, x, right=True) - 1
+    a, b = value[low].double(), value[(low + 1).clamp(max=126)].double()
+    n = 4096
+    u = (torch.arange(n).float() + 0.5) / n
+    codes = F_ref.draw_e4m3(x[:, None].expand(-1, n).contiguous(),
+                            u[None].expand(x.numel(), -1).contiguous())
+    assert bool(((codes == low[:, None]) | (codes == low[:, None] + 1)).all())
+    off = codes.view(E4M3).double().square().mean(1) - x.double() ** 2
+    assert bool((off.abs() <= (b * b - a * a) / n + 1e-6 * x ** 2).all())
+
+
 def test_hash_is_even():
     u = F_ref.hash_uniform(torch.arange(1 << 16), 12345)
     # 65536 draws: the mean of uniforms is within 5 sigma = 5 * 0.289 / 256
