@@ -173,6 +173,41 @@ def test_draw_is_right_in_the_mean():
     assert int((codes.amax(1) - codes.amin(1)).max()) == 1
 
 
+@pytest.mark.parametrize("eps", [1e-50, 2.0 ** -127, float("nan")])
+def test_eps_that_float32_does_not_hold_is_refused(eps):
+    x = make([5], "cpu")
+    with pytest.raises(ValueError, match="eps"):
+        A.adamw_step_(x["params"], x["grads"], x["exp_avgs"],
+                      x["exp_avg_sqs"], x["step"], lr=0.1, eps=eps)
+    with pytest.raises(ValueError, match="eps"):
+        A.AdamW([torch.zeros(3)], eps=eps)
+
+
+def least_eps(device, bits):
+    x = make([300], device, bits, step=0, shadows=False)
+    for name in ("grads", "exp_avgs", "exp_avg_sqs"):
+        x[name][0].view(torch.uint8).zero_()
+    p = x["params"][0].clone()
+    for _ in range(2):
+        A.adamw_step_(x["params"], x["grads"], x["exp_avgs"],
+                      x["exp_avg_sqs"], x["step"], lr=0.1, eps=2.0 ** -126,
+                      weight_decay=0.0,
+                      exp_avg_scales=x.get("exp_avg_scales"),
+                      exp_avg_sq_scales=x.get("exp_avg_sq_scales"))
+    assert torch.equal(x["params"][0], p)     # 0 / eps
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_least_eps_divides_zero(bits):
+    least_eps("cpu", bits)
+
+
+@GPU
+@pytest.mark.parametrize("bits", [32, 8])
+def test_least_eps_divides_zero_gpu(bits):
+    least_eps("cuda", bits)
+
+
 @pytest.mark.parametrize("seed", [0, 2, 10, 45, 62, 165])
 def test_draw_is_right_between_its_neighbours(seed):
     """The same at values that lie so near a code that 4096 even draws may

@@ -32,6 +32,7 @@ from . import functional as F_ref
 
 E4M3 = torch.float8_e4m3fn
 BLOCK = 256
+LEAST_EPS = torch.finfo(torch.float32).tiny
 
 
 def _check(lr, betas, eps, weight_decay, max_norm, grad_scale=1.0):
@@ -39,8 +40,11 @@ def _check(lr, betas, eps, weight_decay, max_norm, grad_scale=1.0):
         raise ValueError(f"adamw_step_: lr must not be negative, got {lr}")
     if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
         raise ValueError(f"adamw_step_: betas must be in [0, 1), got {betas}")
-    if not eps > 0:
-        raise ValueError(f"adamw_step_: eps must be positive, got {eps}")
+    if not eps >= LEAST_EPS:
+        # a smaller one is 0 in float32, or 1 / eps is not finite there: a
+        # value that has seen no gradient would become 0 * inf
+        raise ValueError("adamw_step_: eps must be positive, and at least "
+                         f"{LEAST_EPS:.3g}, got {eps}")
     if not weight_decay >= 0:
         raise ValueError("adamw_step_: weight_decay must not be negative, "
                          f"got {weight_decay}")
