@@ -173,6 +173,48 @@ def test_draw_is_right_in_the_mean():
     assert int((codes.amax(1) - codes.amin(1)).max()) == 1
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_lists_that_do_not_fit_are_refused_unchanged(bits):
+    """On the CPU as on the GPU: a gradient of one value is not spread over
+    its parameter, and nothing has moved when a list turns out wrong."""
+    names = ("params", "grads", "exp_avgs", "exp_avg_sqs")
+    scales = ("exp_avg_scales", "exp_avg_sq_scales")
+
+    def refused(change):
+        x = make([10, 300], "cpu", bits)
+        y = clone(x)
+        change(y)
+        keep = clone(y)
+        with pytest.raises(RuntimeError, match="adamw"):
+            A.adamw_step_(*(y[name] for name in names), y["step"], lr=0.1,
+                          shadows=y["shadows"],
+                          **{name: y.get(name) for name in scales})
+        for name, a in y.items():
+            b = keep[name]
+            for t, u in zip(a, b) if isinstance(a, list) else [(a, b)]:
+                assert torch.equal(t.float(), u.float()), name
+
+    def put(name, k, f):
+        return lambda x: x[name].__setitem__(k, f(x[name][k]))
+
+    for name in names + ("shadows",) + (scales if bits == 8 else ()):
+        refused(put(name, 1, lambda t: t[:1]))
+        refused(lambda x: x[name].pop())
+    for name in ("params", "exp_avgs", "exp_avg_sqs"):
+        refused(put(name, 1, lambda t: t.view(torch.uint8).repeat(2)
+                    [::2].view(t.dtype) if t.dtype == E4M3
+                    else t.repeat(2)[::2]))
+    refused(lambda x: x.update(step=x["step"].float()))
+    refused(lambda x: x.update(step=torch.zeros(2, dtype=torch.int64)))
+    refused(lambda x: x["params"].__setitem__(0, x["params"][1][:10]))
+    if bits == 8:
+        for name in scales:
+            refused(lambda x: x.pop(name))
+    else:
+        refused(lambda x: x.update(exp_avg_sq_scales=[torch.zeros(1),
+                                                      torch.zeros(2)]))
+
+
 @pytest.mark.parametrize("eps", [1e-50, 2.0 ** -127, float("nan")])
 def test_eps_that_float32_does_not_hold_is_refused(eps):
     x = make([5], "cpu")

@@ -56,6 +56,44 @@ def _check(lr, betas, eps, weight_decay, max_norm, grad_scale=1.0):
                          f"{grad_scale}")
 
 
+def _check_lists(params, grads, exp_avgs, exp_avg_sqs, step, m_scales,
+                 v_scales, shadows):
+    """What the eager math cannot do, before anything is written; the
+    kernels' host side has checks of its own."""
+    def check(ok, what):
+        if not ok:
+            raise RuntimeError(f"adamw_step_: {what}")
+
+    bits8 = len(exp_avgs) > 0 and exp_avgs[0].dtype == E4M3
+    check(bits8 == (m_scales is not None) == (v_scales is not None),
+          "states in 8 bits need exp_avg_scales and exp_avg_sq_scales, "
+          "states in 32 bits have none")
+    lists = {"grads": grads, "exp_avgs": exp_avgs, "exp_avg_sqs": exp_avg_sqs,
+             "exp_avg_scales": m_scales, "exp_avg_sq_scales": v_scales,
+             "shadows": shadows, "params": params}
+    lists = {name: x for name, x in lists.items() if x is not None}
+    check(all(len(x) == len(params) for x in lists.values()),
+          "the lists differ in length")
+    check(step.dtype == torch.int64 and step.numel() == 1,
+          "step must be one int64")
+    written = [step]
+    for name, tensors in lists.items():
+        for k, x in enumerate(tensors):
+            if x is None and name == "shadows":
+                continue
+            n = params[k].numel()
+            n = -(-n // BLOCK) if name.endswith("scales") else n
+            check(x.numel() == n, f"{name}[{k}] has {x.numel()} values, "
+                  f"expected {n}")
+            # the eager math reads gradients, and writes copies, of any order
+            check(name in ("grads", "shadows") or x.is_contiguous(),
+                  f"{name}[{k}] must be contiguous")
+            if n and name != "grads":
+                written.append(x)
+    check(len({x.data_ptr() for x in written}) == len(written),
+          "parameters, states or shadows share memory")
+
+
 @torch.no_grad()
 def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr,
                 betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
@@ -80,15 +118,8 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr,
             params, grads, exp_avgs, exp_avg_sqs, step, lr, betas[0],
             betas[1], eps, weight_decay, max_norm, grad_scale,
             exp_avg_scales, exp_avg_sq_scales, shadows)
-    lists = [grads, exp_avgs, exp_avg_sqs] + [
-        x for x in (exp_avg_scales, exp_avg_sq_scales, shadows)
-        if x is not None]
-    if any(len(x) != len(params) for x in lists):
-        raise RuntimeError("adamw_step_: the lists differ in length")
-    if (exp_avgs[0].dtype == E4M3) != (exp_avg_scales is not None):
-        raise RuntimeError("adamw_step_: states in 8 bits need "
-                           "exp_avg_scales and exp_avg_sq_scales, states in "
-                           "32 bits have none")
+    _check_lists(params, grads, exp_avgs, exp_avg_sqs, step, exp_avg_scales,
+                 exp_avg_sq_scales, shadows)
     return F_ref.adamw_step_(
         params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps,
         weight_decay, max_norm, grad_scale, exp_avg_scales,
