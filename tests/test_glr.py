@@ -189,6 +189,19 @@ def test_refusals_eager():
             call()
 
 
+def test_no_steps_and_no_rows_eager():
+    for T, B, H in [(0, 3, 4), (5, 0, 4), (5, 3, 0), (0, 0, 0)]:
+        gates, c0, dh, dcT, _ = make(T, B, H, torch.float32, "cpu")
+        h, cT, dgates, dc0 = check(gates, c0, dh, dcT, None)
+        assert h.shape == (T, B, H) and dgates.shape == gates.shape
+        d, dc0 = G.glr_backward(None, None, gates, None, None)
+        assert d.shape == gates.shape and not dc0.any()
+        c = c0.clone().requires_grad_()
+        h, cT = G.glr(gates, c)
+        (cT * dcT).sum().backward()
+        assert c.grad.shape == c0.shape
+
+
 def test_step_is_the_scan_eager():
     gates, c0, *_ = make(9, 4, 6, torch.float32, "cpu")
     h, cT, _ = G.glr_forward(gates, c0)

@@ -106,7 +106,9 @@ def glr_backward(dh, dcT, gates, c0, marks, lengths=None, *, out=None):
         h, cT = F_ref.glr_layer(g, c, lengths)
         dh = torch.zeros_like(h) if dh is None else dh
         dcT = torch.zeros_like(cT) if dcT is None else dcT
-        dg, dc0 = torch.autograd.grad((h, cT), (g, c), (dh, dcT),
+        ends = ((h, dh), (cT, dcT))[gates.size(0) == 0:]  # no steps, no h
+        dg, dc0 = torch.autograd.grad([x for x, _ in ends], (g, c),
+                                      [d for _, d in ends],
                                       allow_unused=True)
     dg = torch.zeros_like(g) if dg is None else dg
     return (dg if out is None else out.copy_(dg)), dc0
