@@ -189,6 +189,28 @@ def test_refusals_eager():
             call()
 
 
+def test_refusals_eager_of_outputs_and_gradients():
+    """Those of the kernels: nothing is spread over a larger `out`, and no
+    type is changed on the way."""
+    gates, c0, dh, dcT, _ = make(4, 3, 2, torch.float32, "cpu")
+    for call in (
+            lambda: G.glr_forward(gates, c0, out=torch.zeros(5, 4, 3, 2)),
+            lambda: G.glr_forward(gates, c0, out=torch.zeros(4, 3, 3)),
+            lambda: G.glr_forward(gates, c0, out=dh.half()),
+            lambda: G.glr_backward(dh, dcT, gates, c0, None,
+                                   out=torch.zeros(2, 4, 3, 8)),
+            lambda: G.glr_backward(dh, dcT, gates, c0, None,
+                                   out=gates.double()),
+            lambda: G.glr_backward(dh.half(), dcT, gates, c0, None),
+            lambda: G.glr_backward(dh[:2], dcT, gates, c0, None)):
+        with pytest.raises(RuntimeError, match="glr"):
+            call()
+    h, d = torch.zeros_like(dh), torch.zeros_like(gates)
+    assert G.glr_forward(gates, c0, out=h)[0] is h
+    assert G.glr_backward(dh, dcT, gates, c0, None, out=d)[0] is d
+    assert h.any() and d.any()
+
+
 def test_no_steps_and_no_rows_eager():
     for T, B, H in [(0, 3, 4), (5, 0, 4), (5, 3, 0), (0, 0, 0)]:
         gates, c0, dh, dcT, _ = make(T, B, H, torch.float32, "cpu")

@@ -71,6 +71,16 @@ def _check_lengths(op, gates, lengths):
                            f"{list(lengths.shape)}")
 
 
+def _check_like_h(op, name, x, gates, width):
+    if x is None:
+        return
+    want = (gates.size(0), gates.size(1), width)
+    if tuple(x.shape) != want or x.dtype != gates.dtype:
+        raise RuntimeError(f"{op}: {name} must be {list(want)} of the gates' "
+                           f"type {gates.dtype}, got {list(x.shape)} of "
+                           f"{x.dtype}")
+
+
 def glr_forward(gates, c0=None, lengths=None, *, training=False, out=None):
     """``(h, cT, marks)`` without autograd. ``marks`` is what
     ``glr_backward`` needs of the forward pass, None unless ``training``.
@@ -79,6 +89,7 @@ def glr_forward(gates, c0=None, lengths=None, *, training=False, out=None):
         return _C.ext().glr_forward(gates, c0, lengths, training, out)
     _check_eager("glr_forward", gates, 3, c0=c0)
     _check_lengths("glr_forward", gates, lengths)
+    _check_like_h("glr_forward", "out", out, gates, gates.size(2) // 4)
     with torch.no_grad():
         h, cT = F_ref.glr_layer(gates, c0, lengths)
     if out is not None:
@@ -98,6 +109,8 @@ def glr_backward(dh, dcT, gates, c0, marks, lengths=None, *, out=None):
         return _C.ext().glr_backward(dh, dcT, gates, c0, marks, lengths, out)
     _check_eager("glr_backward", gates, 3, c0=c0, dcT=dcT)
     _check_lengths("glr_backward", gates, lengths)
+    _check_like_h("glr_backward", "dh", dh, gates, gates.size(2) // 4)
+    _check_like_h("glr_backward", "out", out, gates, gates.size(2))
     with torch.enable_grad():
         g = gates.detach().requires_grad_()
         c = (torch.zeros(gates.size(1), gates.size(2) // 4,
