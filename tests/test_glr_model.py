@@ -526,3 +526,100 @@ def test_gave_up_is_checked():
             e.glr_forward(gates, None, None, False, None, bad)
     with pytest.raises(RuntimeError, match="set_glr_polls"):
         e.set_glr_polls(-1)
+
+
+@GPU
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("cell", ["glr", "lstm"])
+def test_hip_shadows_after_adamw_are_those_of_the_masters(cell, bits):
+    """What a step leaves (copies, transposes, packs, folded biases) against
+    what the masters give, tensor by tensor and in the next scores."""
+    torch.manual_seed(0)
+    m = Model(203, 72, 2, 0.0, 0.1, engine="hip", cell=cell).cuda()
+    opt = AdamW(m.parameters(), bits=bits)
+    for step in range(3):
+        x, y = batch(11, 4, 203, seed=step, device="cuda")
+        m.zero_grad(set_to_none=True)
+        scores, _ = m(x, m.state_init(4))
+        trainer.nll_loss(scores, y).backward()
+        trainer.adamw_step(m, opt, 1e-2, 0.5)
+    hm = m._hip_model
+    assert hm._shadows_fresh
+
+    def shadows():
+        out = {"emb": hm.emb_W, "fc": hm.fc.W, "fcT": hm.fc.WT}
+        for k, rt in enumerate(hm.layers):
+            for name in ("Wx", "WxT") + (
+                    ("Wh", "WhT", "WhP", "WhTP", "bias_sum")
+                    if cell == "lstm" else ()):
+                out[f"{name}{k}"] = getattr(rt, name)
+        return {name: t.clone() for name, t in out.items()}
+
+    def forward():
+        with torch.no_grad():
+            return m(x, m.state_init(4))[0].clone()
+
+    left, a = shadows(), forward()
+    hm.refresh_shadows()
+    for name, t in shadows().items():
+        assert torch.equal(left[name], t), name
+    assert torch.equal(a, forward())
+    # the update was not lost on the way: a plain copy of the new masters
+    assert torch.equal(left["emb"], m.embed.W.detach().bfloat16())
+    assert torch.equal(left["Wx1"], m.rnns[1].W_x.detach().bfloat16())
+
+
+@GPU
+@pytest.mark.parametrize("T,B,H", [(4099, 1, 72), (2048, 5, 136)])
+def test_hip_model_follows_eager_over_a_long_text(monkeypatch, T, B, H):
+    """Scores, states and gradients of a window that is a chain of tiles.
+
+    A weight's gradient is the sum of what the rows (tokens) add to it. Their
+    signs differ and their roundings are alike (the probabilities of all rows
+    are near 1 / 203, and are rounded alike), so that the sum may be off by
+    far more than GRADS of itself. Here the gate gradients are held to GRADS
+    row by row, and the sums to what the rows that went into them give: a
+    matrix instruction adds 32 rows to a float32 sum, a column sum 64, with
+    2^-24 of the sum at each addition: under (64 + T B / 32) 2^-24 of the
+    terms' magnitudes."""
+    eager = model(vocab=203, hidden=H).cuda()
+    hip = model("hip", vocab=203, hidden=H).cuda()
+    hip.load_state_dict(eager.state_dict())
+    x, y = batch(T, B, 203, device="cuda")
+    layer, gates, inputs = F_ref.glr_layer, [], []
+
+    def recorded(g, c0):
+        g.retain_grad()
+        gates.append(g)
+        return layer(g, c0)
+
+    def kept(cur, *rest):
+        inputs.append(cur.detach().clone())
+        return hip_layer(cur, *rest)
+
+    hm = hip.hip()
+    hip_layer = hm._glr_layer
+    monkeypatch.setattr(hm, "_glr_layer", kept)
+    out = []
+    for m in (eager, hip):
+        with monkeypatch.context() as patch:
+            if m is eager:
+                patch.setattr(F_ref, "glr_layer", recorded)
+            scores, states = m(x, m.state_init(B))
+        F_ref.nll_loss(scores, y).backward()
+        out.append((scores, states))
+    (s0, st0), (s1, st1) = out
+    hm.check_aborts()
+    assert rel(s1, s0) < SCORES
+    for (_, c0), (_, c1) in zip(st0, st1):
+        assert rel(c1, c0) < SCORES
+    bound = (64 + T * B / 32) * 2.0 ** -24
+    for k, rt in enumerate(hm.layers):
+        d = rt.ws.dG.view(T * B, -1).double()
+        assert rel(d, gates[k].grad.view(T * B, -1)) < GRADS, k
+        xs = inputs[k].view(T * B, -1).double()
+        for got, want, size in (
+                (hip.rnns[k].b_x, d.sum(0), d.abs().sum(0)),
+                (hip.rnns[k].W_x, d.t() @ xs, d.t().abs() @ xs.abs())):
+            off = (got.grad.double() - want).abs()
+            assert bool((off <= bound * size).all()), k
