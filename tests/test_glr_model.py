@@ -623,3 +623,32 @@ def test_hip_model_follows_eager_over_a_long_text(monkeypatch, T, B, H):
                 (hip.rnns[k].W_x, d.t() @ xs, d.t().abs() @ xs.abs())):
             off = (got.grad.double() - want).abs()
             assert bool((off <= bound * size).all()), k
+
+
+@GPU
+@pytest.mark.parametrize("cell", ["glr", "lstm"])
+def test_hip_side_stream_reads_what_is_freed(monkeypatch, cell):
+    """The projection's weight gradient on a side stream, while the main one
+    goes on to allocate: its inputs are not handed out again before."""
+    def grads(side):
+        monkeypatch.setenv("ZAREMBA_AMD_SIDE_STREAM", side)
+        torch.manual_seed(0)
+        m = Model(503, 200, 1, 0.0, 0.1, engine="hip", cell=cell).cuda()
+        out = []
+        for seed in range(4):
+            x, y = batch(35, 20, 503, seed=seed, device="cuda")
+            m.zero_grad()
+            scores, states = m(x, m.state_init(20))
+            loss = trainer.nll_loss(scores, y)
+            del scores, states
+            loss.backward()
+            rooms = [torch.full((35 * 20, k), 1e30, device="cuda")
+                     for k in (100, 200, 503, 503)]
+            torch.cuda.synchronize()
+            out.append([m.fc.W.grad.clone(), m.rnns[0].W_x.grad.clone()])
+            del rooms
+            m._hip_model.side_events.clear()
+        return out
+
+    assert all(torch.equal(a, b) for xs, ys in zip(grads("0"), grads("1"))
+               for a, b in zip(xs, ys))

@@ -151,6 +151,11 @@ class LinearFn(torch.autograd.Function):
             ev0 = torch.cuda.Event()
             ev0.record()  # dsc / x / dscores ready on the main stream
             side.wait_event(ev0)
+            # these may be freed when this returns: the allocator must not
+            # hand their memory to the main stream before the side stream
+            # has read it
+            x.record_stream(side)
+            dscores_c.record_stream(side)
             with torch.cuda.stream(side):
                 dW, db = dw_family()
                 ev1 = torch.cuda.Event()
