@@ -399,6 +399,24 @@ def test_a_saved_state_stays_as_it_was(bits):
     assert torch.equal(steps(), first)
 
 
+@pytest.mark.parametrize("bits,name", [
+    (32, "exp_avg_sqs"), (8, "exp_avg_sqs"), (8, "exp_avg_sq_scales")])
+def test_states_of_another_model_change_nothing(bits, name):
+    p = torch.nn.Parameter(torch.randn(300))
+    opt = A.AdamW([p], bits=bits)
+    p.grad = torch.randn(300)
+    opt.step(0.01)
+    other, keep = opt.state_dict(), opt.state_dict()
+    p.grad = torch.randn(300)
+    for x in other["exp_avgs"]:
+        x.view(torch.uint8).fill_(1)
+    other[name] = [x[:1] for x in other[name]]
+    with pytest.raises(ValueError, match=name):
+        opt.load_state_dict(other)
+    for a, b in zip(opt.state_dict()["exp_avgs"], keep["exp_avgs"]):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 # ---------------------------------------------------------------------------
 # kernels
 # ---------------------------------------------------------------------------

@@ -187,13 +187,14 @@ class AdamW:
         if state["bits"] != self.bits:
             raise ValueError(f"AdamW: the saved states have {state['bits']} "
                              f"bits, these {self.bits}")
-        for name in self._LISTS:
-            mine, saved = getattr(self, name), state[name]
-            if mine is None:
-                continue
-            if [t.shape for t in mine] != [t.shape for t in saved]:
+        names = [name for name in self._LISTS
+                 if getattr(self, name) is not None]
+        for name in names:  # all of them, before one is written
+            if ([t.shape for t in getattr(self, name)]
+                    != [t.shape for t in state[name]]):
                 raise ValueError(f"AdamW: the saved {name} are of another "
                                  "model")
-            for a, b in zip(mine, saved):
+        for name in names:
+            for a, b in zip(getattr(self, name), state[name]):
                 a.copy_(b)
         self.step_count.copy_(state["step_count"])
