@@ -193,3 +193,32 @@ def test_steps_within_their_roundings(small):
         value, bound = want["h"]
         assert outside(h, value[t], bound[t]) == 0, t
     assert outside(c, *want["cT"]) == 0
+
+
+@GPU
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16,
+                                   torch.float16])
+@pytest.mark.parametrize("T,B,H", [(35, 6, 40), (128, 5, 9), (700, 6, 70)])
+def test_padded_rows_within_their_roundings(dtype, T, B, H):
+    """Each row of a padded batch, batch first, as the window that it is."""
+    gen = torch.Generator().manual_seed(1)
+    gates, c0, dh, dcT = make(T, B, H, "cuda", dtype)
+    first = lambda x: x.transpose(0, 1).contiguous().transpose(0, 1)  # noqa
+    gates, dh = first(gates), first(dh)
+    ends = torch.randint(1, T + 1, (B,), generator=gen).tolist()
+    ends[0], ends[-1] = 0, T
+    for b, n in enumerate(ends):
+        gates[n:, b], dh[n:, b] = float("nan"), float("inf")
+    lengths = torch.tensor(ends, device="cuda")
+    h, cT, marks = G.glr_forward(gates, c0, lengths, training=True)
+    dgates, dc0 = G.glr_backward(dh, dcT, gates, c0, marks, lengths)
+    for b, n in enumerate(ends):
+        row = slice(b, b + 1)
+        assert not h[n:, b].any() and not dgates[n:, b].any()
+        if n == 0:
+            assert torch.equal(cT[b], c0[b]) and torch.equal(dc0[b], dcT[b])
+            continue
+        want = bounds(gates[:n, row], c0[row], dh[:n, row], dcT[row])
+        for name, got in (("h", h[:n, row]), ("cT", cT[row]),
+                          ("dgates", dgates[:n, row]), ("dc0", dc0[row])):
+            assert outside(got, *want[name]) == 0, (name, b)
