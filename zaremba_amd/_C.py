@@ -51,7 +51,7 @@ def ext():
 
 def force_eager_env() -> bool:
     # Asked at every call of an operator: 0.6 us through os.environ, which
-    # sets the process's environment, too; 0.2 from there.
+    # sets the process's environment, too; 0.1 from there.
     if _ext is not None:
         return _ext.force_eager_env()
     return os.environ.get("ZAREMBA_AMD_FORCE_EAGER", "0") == "1"

@@ -15,9 +15,9 @@
 // Two launches: the sum of squares (the norm is of all gradients, so they are
 // read twice), and the update, in which a wave of each block first adds up the
 // partial sums while all of the block's loads are in flight. At 66.0M
-// parameters with bf16 shadows they take 416 us in 32 bits (2.25 GB with the
+// parameters with bf16 shadows they take 418 us in 32 bits (2.25 GB with the
 // second reading, 5.4 TB/s, more than the 5.2 of a copy as a cache holds some of
-// it), and 279 us in 8 bits (1.46 GB, 5.2 TB/s; some 62 vector instructions a
+// it), and 272 us in 8 bits (1.46 GB, 5.4 TB/s; some 62 vector instructions a
 // value).
 //
 // Sums and the arithmetic of an update are in the order of the formulas, each
@@ -183,6 +183,9 @@ DEV_INLINE float clip_scale(const AdamwScalars& s, const AdamwWork& w,
   return scale;
 }
 
+// A published 32-bit mixer (C. Wellons, "Prospecting for Hash Functions",
+// 2018), fed with multiples of two primes (the first two of Y. Collet's 32-bit
+// xxHash).
 constexpr unsigned HASH_INDEX = 0x9E3779B1u, HASH_STEP = 0x85EBCA77u;
 
 DEV_INLINE float hash_uniform(unsigned x) {

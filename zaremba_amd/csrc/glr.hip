@@ -48,7 +48,7 @@ DEV_INLINE float sigmoid_f(float x) { return rcp_f(1.f + exp2_f(x * -LOG2E)); }
 
 // 1 - exp(-2|x|) cancels for small x: its error is 2^-24 of 1. A value under
 // SMALL is therefore taken from the series x - x^3 / 3 + 2 x^5 / 15, whose next
-// term is under 2^-22 of it, and tanh is off by at most 16 * 2^-24 of its value.
+// term is under 2^-22 of it, and tanh is off by at most 16 * 2^-24 of itself.
 // Where gates and h have 16 bits x itself does, a third of whose square is
 // under 2^-17, and the bound is 330 * 2^-24, a twelfth of half a step of f16:
 // at 65536 x 1 x 1500 bf16 this costs 249 -> 254 us forward, the series 279.
@@ -176,7 +176,8 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 }
 
 // A window of more than one tile is a block for each tile, all in flight at
-// once, that hand the state on. Slot r, the r-th tile in the order of the
+// once, that hand the state on: a scan in one pass with decoupled look-back
+// (D. Merrill and M. Garland, 2016). Slot r, the r-th tile in the order of the
 // scan, has a word for each channel. It first publishes its (A, C) there and,
 // once it knows the state before it, the state behind it instead, marked by
 // A = -1. A wave looks back over the slots before its own, DEPTH of them at a
@@ -193,9 +194,9 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 // chain ends, or in the backward pass begins, with the tile before. Rows of
 // random lengths, forward / backward in tiles of 8 waves: 133 / 243 us against
 // 155 / 279 with such tiles in the chain at 512 x 80 x 1500, 28 / 55 against
-// 35 / 59 at 1001 x 17 x 651. Their reads are half of all; an XCD whose rows are short then waits for
-// the others, and dealing groups out in smaller pieces costs as much in lines
-// that two XCDs read.
+// 35 / 59 at 1001 x 17 x 651. Their reads are half of all; an XCD whose rows
+// are short then waits for the others, and dealing groups out in smaller pieces
+// costs as much in lines that two XCDs read.
 //
 // Blocks take their slots from counters as they start. A block therefore
 // waits only for blocks that run already, and these only for earlier ones:
@@ -208,21 +209,24 @@ DEV_INLINE float compose(float c, const Pair (*pairs)[64], int from, int to) {
 // seldom whole cache lines, and the other halves are then met in the same L2.
 // (Blocks go round the XCDs in turn; no result depends on it.) Windows of one
 // tile have the same shares: in us, against groups in the blocks' order, 35 x
-// 20 x 1500 bf16 6.6 / 7.3 against 6.6 / 9.3 forward / backward, 100 x 20 x 1500
-// 9.3 / 17.4 against 12.0 / 21.5, 35 x 128 x 1500 17 / 33 against 22 / 45, rows of
-// whole lines (64 x 64 x 1024) the same. In a chain with fewer groups each has a counter of its own, as the blocks of one would
-// queue at one address (14 ns a slot) and an XCD would have 3 groups or less.
+// 20 x 1500 bf16 6.6 / 7.3 against 6.6 / 9.3 forward / backward, 100 x 20 x
+// 1500 9.3 / 17.4 against 12.0 / 21.5, 35 x 128 x 1500 17 / 33 against 22 / 45,
+// rows of whole lines (64 x 64 x 1024) the same. In a chain with fewer groups
+// each has a counter of its own, as the blocks of one would queue at one
+// address (14 ns a slot) and an XCD would have 3 groups or less.
 // Measured in us, forward / backward in tiles of 8 waves, bf16, H = 1500: with
 // a counter a group against shares, 23.4 groups x 65536 steps 250 / 537 against
 // 276 / 578 (one counter for all: 260 / 545), 15.6 x 16384 (H = 1000) 53 / 90
 // against 52 / 99, but 94 x 4096 69 / 141 against 65 / 120 and 375 x 1024 70 /
 // 146 against 62 / 113.
 //
-// At T = 65536, B = 1, H = 1500, bf16 this takes 250 us forward (983 MB, 3.9
-// TB/s of the 5.2 that a copy reaches) and 537 backward (1770 MB, 3.3 TB/s);
-// with rows of whole lines, H = 1472, 201 (4.8 TB/s) and 353 (4.9). The rest is
-// lines that two XCDs read: 1.6 and 1.8 times the bytes at H = 1500. Vector
-// instructions take half of either. Before, finding the (A, C) of long chunks
+// At T = 65536, B = 1, H = 1500, bf16 this takes 255 us forward (983 MB, 3.9
+// TB/s of the 5.2 that a copy reaches) and 518 backward (1770 MB, 3.4 TB/s);
+// with rows of whole lines, H = 1472, 209 (4.6 TB/s) and 353 (4.9). At H = 1500
+// two XCDs read the same lines, 1.4 and 1.75 times the bytes to be read. That
+// is not what bounds the backward pass: shares for XCDs take a quarter of its
+// read bytes away and no time. What does is not known. Vector instructions
+// take half of either. Before, finding the (A, C) of long chunks
 // in a launch of its own, which reads three gates twice, took 360 and 680, and
 // a block that loops over its tiles 2380 and 4500.
 constexpr unsigned ABSENT = 0xffffffffu;
@@ -341,8 +345,8 @@ struct Chain {
 
   // The state before `slot`, to all waves; the one behind it through `last`.
   DEV_INLINE float hand_on(int slot, const Channel& ch, float A, float C,
-                           const float* start, float* lds, Pair (*seen)[64], float* last,
-                           int w) const {
+                           const float* start, float* lds, Pair (*seen)[64],
+                           float* last, int w) const {
     if (w == 0) {
       publish(slot, ch, A, C);
       const float c = look_back(slot, ch, start ? start[ch.state] : 0.f, seen);
@@ -532,8 +536,8 @@ __global__ __launch_bounds__(64 * W) void glr_bwd_kernel(GlrArgs a) {
         sum = p.A * sum + p.C;
         whole *= p.A;
       }
-    carry = Chain(a).hand_on(tiles - 1 - tile, ch, whole, sum, a.dcT, handed, seen,
-                             begin == 0 ? a.dc0 : nullptr, w);
+    carry = Chain(a).hand_on(tiles - 1 - tile, ch, whole, sum, a.dcT, handed,
+                             seen, begin == 0 ? a.dc0 : nullptr, w);
   } else {
     carry = a.dcT ? a.dcT[ch.state] : 0.f;
   }
@@ -581,23 +585,25 @@ void by_type(GlrType type, F f) {
 // Steps of a wave, and waves of a block. Up to 128 steps are one tile of waves
 // with 8 steps each, backward up to 64 of waves with 4: more waves to hide the
 // one round of loads. 35 x 20 x 1500 bf16 takes 7.3 us with 4 against 8.3, 16 x
-// 64 x 1500 8.1 against 9.5, but 64 x 128 x 650 23 against 21; forward 4 measure
-// 6.6 against 6.4, 17 against 16 at 35 x 128 x 1500, 14.5 against 12.6 at 64 x 128
-// x 650. From 65 steps on a chain would take 13 / 18 us at 65 x 20 x 1500 against
-// 7.2 / 11.4, and 58 / 116 against 57 / 125 at 128 x 128 x 1500.
+// 64 x 1500 8.1 against 9.5, but 64 x 128 x 650 23 against 21; forward 4
+// measure 6.6 against 6.4, 17 against 16 at 35 x 128 x 1500, 14.5 against 12.6
+// at 64 x 128 x 650. From 65 steps on a chain would take 13 / 18 us at 65 x 20
+// x 1500 against 7.2 / 11.4, and 58 / 116 against 57 / 125 at 128 x 128 x 1500:
+// there alone, backward with many channels, the one threshold is not the best.
 //
 // A chain's tiles are 128 steps forward, 64 backward, of 8 waves. 16 waves with
 // 8 steps measured 218 us against 200 forward at 65536 x 1 x 1472, 4 waves with
 // 16 566 against 545 backward at 65536 x 1 x 1500. Forward with MANY_GROUPS, a
 // group for each CU, tiles are 64 steps of 4 waves: blocks end sooner, and more
-// of them wait while others load. 300 x 64 x 650 takes 34 us against 39, 512 x 80
-// x 1500 135 against 147 and with random lengths 110 against 127, 1024 x 16 x 1500
-// 56 against 60, but 256 x 20 x 1500 21.8 against 21.3; with fewer groups 65536 x
-// 1 x 1500 273 against 256, 8192 x 2 x 1024 f32 73 against 70. Backward the same
-// costs 3 to 15 %. Blocks that loop over tiles, which need no chain, measured
-// from 256 steps on up to four times a chain's time where channels are few (23
-// groups, 512 steps: 20 / 33 us against 10 / 14) and 1.1 to 1.4 times where they
-// are many (1875 groups, 512 steps: 161 / 401 against 153 / 292).
+// of them wait while others load. 300 x 64 x 650 takes 34 us against 39, 512 x
+// 80 x 1500 135 against 147 and with random lengths 110 against 127, 1024 x 16
+// x 1500 56 against 60, but 256 x 20 x 1500 21.8 against 21.3; with fewer
+// groups 65536 x 1 x 1500 273 against 256, 8192 x 2 x 1024 f32 73 against 70.
+// Backward the same costs 3 to 15 %. (All before the selects of small_tanh, up
+// to 2 % on either side.) Blocks that loop over tiles, which need no chain,
+// measured from 256 steps on up to four times a chain's time where channels are
+// few (23 groups, 512 steps: 20 / 33 us against 10 / 14) and 1.1 to 1.4 times
+// where they are many (1875 groups, 512 steps: 161 / 401 against 153 / 292).
 constexpr int TILE_STEPS = 8, SHORT_STEPS = 4, TILE_WAVES = 16;
 constexpr int FWD_STEPS = 16, BWD_STEPS = 8, CHAIN_WAVES = 8;
 constexpr int MANY_GROUPS = 256, MANY_WAVES = 4;

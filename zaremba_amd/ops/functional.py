@@ -199,7 +199,8 @@ def _e4m3_scales(x: torch.Tensor):
 
 
 def hash_uniform(index: torch.Tensor, step) -> torch.Tensor:
-    """Numbers in [0, 1) with 24 bits, from a 32-bit mixing hash."""
+    """Numbers in [0, 1) with 24 bits, from a 32-bit mixing hash
+    (csrc/adamw.hip names it)."""
     low = 0xFFFFFFFF
     x = (index.long() * 0x9E3779B1 + step * 0x85EBCA77) & low
     x = ((x ^ (x >> 16)) * 0x7FEB352D) & low
